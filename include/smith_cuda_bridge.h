@@ -82,7 +82,12 @@ void* smith_compile_source(void* ctx, const char* source, char** error_out);
  * "matmul_simple_f16" (buffers 0=A [M,K], 1=B [K,N], 2=C [M,N]; bytes at 3 =
  * uint32 {M,N,K}) and "matmul_batched", "matmul_batched_f16" (leading batch
  * dimension on all three; bytes at 3 = uint32 {M,N,K,batch}), as
- * src/ops/matmul.js:26-52,70-79 binds them.  NULL for anything else. */
+ * src/ops/matmul.js:26-52,70-79 binds them; the int8 family "quantize_int8[_f16]"
+ * (buffers 0=W, 1=packed out; bytes at 2 = uint32 {K,N,experts}), "matmul_int8[_f16]"
+ * (buffers 0=A, 1=packed B, 2=C; bytes at 3 = uint32 {M,N,K}), "matmul_int8_grouped[_f16]"
+ * (the same and 4=offsets, optionally 5=position, 6=order; bytes at 3 = uint32
+ * {rows,N,K,experts,fan}) and "group_rows" (buffers 0=ids, 1=offsets, 2=order,
+ * 3=position; bytes at 4 = uint32 {rows,experts}).  NULL for anything else. */
 void* smith_create_pipeline(void* ctx, void* library, const char* fn_name);
 
 typedef struct SmithEncoder SmithEncoder;
@@ -204,6 +209,42 @@ int32_t smith_qmatmul(void* ctx, uint32_t kind, void* a, void* b, void* c, uint6
 #define SMITH_DENSE_TENSOR_FAST 3u
 int32_t smith_matmul(void* ctx, uint32_t dtype, void* a, void* b, void* c, uint64_t M, uint64_t N, uint64_t K,
                      uint64_t batch, uint32_t path);
+/* Products in 8-bit integers with a scale per token and per channel (no counterpart in the reference),
+ * for one weight matrix or for rows sorted by expert with a matrix each.  For a vector x of finite values
+ *     scale(x) = max|x| / 127,  code(x)[k] = round-half-to-even(127 x[k] / max|x|)
+ * (the quotients as real numbers; a vector of zeros has scale 0 and codes 0; one that holds an infinity or
+ * a NaN has scale NaN, so its outputs are NaN, and no others).  Then
+ *     c[m, n] = (sum_k code(a_m)[k] * code(w_n)[k]) * scale(a_m) * scale(w_n)
+ * with the sum exact (1 <= K <= 131072), f32(sum) * f32 scale(a_m) * f32 scale(w_n) in that order (in f64,
+ * where a scale is outside [2^-60, 2^60] and not 0), then rounded to c's type.
+ * dtype (SMITH_DTYPE_F32 / _F16) is that of a and c.
+ *
+ * smith_int8_pack packs weights w [experts][K][N] (f32 or f16, channels are columns) into
+ * smith_int8_packed_bytes(K, N, experts) bytes, which must start on 16 bytes; 0 bytes: sizes not taken.
+ * N is at most 2^22, experts at most 1024.
+ * smith_int8_matmul: c[M,N] = a[M,K] x w.  Row pitches lda, ldc in elements; 0: K and N.  c may overlap a.
+ * smith_int8_matmul_grouped: offsets i32 [experts + 1], rising; sorted rows offsets[e] .. offsets[e + 1]
+ * meet the matrix of expert e.  Rows of c that belong to no expert are left as they are.
+ *     position NULL: a holds the `rows` rows in sorted order (fan is 1);
+ *     position i32 [rows]: a holds rows / fan rows, row t stands at the sorted places
+ *         position[t * fan] .. position[t * fan + fan - 1] (each place below offsets[experts] named once);
+ *     order NULL: c is in sorted order; order i32 [rows]: sorted row j is row order[j] of c (different rows).
+ *     Places and rows outside [0, rows) are skipped; offsets outside [0, rows] are clamped.
+ * smith_group_rows makes the three lists on the device from ids i32 [rows] (a stable sort by id; ids
+ * outside [0, experts) belong to no expert and come last): offsets [experts + 1], order [rows],
+ * position [rows].  For `top` experts per token, ids [tokens][top] gives lists that fit fan = top.
+ * All are asynchronous on the context's stream and may be captured in a graph once a call of the size
+ * has been made outside the capture (scratch of rows * (K rounded up to 128, + 4) bytes and partial sums;
+ * it grows as needed, and a block that a captured graph uses is kept until smith_destroy). */
+uint64_t smith_int8_packed_bytes(uint64_t K, uint64_t N, uint64_t experts);
+int32_t smith_int8_pack(void* ctx, uint32_t dtype, void* w, void* out, uint64_t K, uint64_t N, uint64_t experts);
+int32_t smith_int8_matmul(void* ctx, uint32_t dtype, void* a, void* w, void* c, uint64_t M, uint64_t N, uint64_t K,
+                          uint64_t lda, uint64_t ldc);
+int32_t smith_int8_matmul_grouped(void* ctx, uint32_t dtype, void* a, void* w, void* offsets, void* c, uint64_t rows,
+                                  uint64_t N, uint64_t K, uint64_t experts, uint64_t lda, uint64_t ldc, void* position,
+                                  void* order, uint64_t fan);
+int32_t smith_group_rows(void* ctx, void* ids, void* offsets, void* order, void* position, uint64_t rows,
+                         uint64_t experts);
 /* No counterpart in the reference, whose callers issue one matmul per weight matrix
  * (src/gguf_cache.js:121-171: wq, wk, wv on the same input; gate and up on the same input).
  * c_bufs[i] [M, n_list[i]] = a [M, K] x dequant(b_bufs[i]) for 1 to 4 packed matrices of the same K

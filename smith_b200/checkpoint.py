@@ -7,7 +7,8 @@ weights: quantizing a 70B-shaped stack takes 52 GB of device packing per run,
 loading the packed bytes does not.  Block layouts are the ones the matmul
 kernels read (24-byte Q4 blocks, 34-byte Q8 blocks, block (g, col) at
 (g * N + col) * block_bytes), so a loaded record goes straight to
-matmulQ4 / matmulQ8.
+matmulQ4 / matmulQ8.  Records of quantizeInt8 (kind "i8") are kept the same way: their packed bytes as
+they are, with the number of experts instead of the block groups.
 """
 import json
 
@@ -24,17 +25,30 @@ def _block_bytes(kind):
         return GROUP_BYTES
     if kind == "q8":
         return Q8_BLOCK_BYTES
-    raise ValueError(f"saveQuantized: kind must be 'q4' or 'q8', got {kind!r}")
+    raise ValueError(f"saveQuantized: kind must be 'q4', 'q8' or 'i8', got {kind!r}")
+
+
+def _int8_bytes(fields):
+    return device.int8PackedBytes(int(fields["K"]), int(fields["N"]), int(fields["experts"]))
 
 
 def saveQuantized(records, path):
     """``records``: {name: (kind, record)} with record = the {buffer, K, N, groups, totalBytes} of
-    quantizeQ4 / quantizeQ8.  Writes ``path.json`` and ``path.bin``."""
+    quantizeQ4 / quantizeQ8 or the {buffer, K, N, experts, totalBytes} of quantizeInt8.  Writes ``path.json`` and ``path.bin``."""
     entries, offset = [], 0
     with open(path + ".bin", "wb") as f:
         for name, (kind, rec) in records.items():
-            bb = _block_bytes(kind)
             total = int(rec["totalBytes"])
+            if kind == "i8":
+                if total != _int8_bytes(rec):
+                    raise ValueError(f"saveQuantized: {name}: totalBytes does not match K, N and experts")
+                device.synchronize()
+                f.write(device.download(rec["buffer"], total, np.uint8).tobytes())
+                entries.append({"name": name, "kind": kind, "K": int(rec["K"]), "N": int(rec["N"]),
+                                "experts": int(rec["experts"]), "totalBytes": total, "offset": offset})
+                offset += total
+                continue
+            bb = _block_bytes(kind)
             if total != int(rec["groups"]) * int(rec["N"]) * bb:
                 raise ValueError(f"saveQuantized: {name}: totalBytes does not match groups * N * {bb}")
             device.synchronize()
@@ -57,11 +71,13 @@ def loadQuantized(path):
         raise ValueError(f"loadQuantized: {path}.bin holds {blob.size} bytes, the manifest says {manifest['totalBytes']}")
     out = {}
     for e in manifest["weights"]:
-        bb = _block_bytes(e["kind"])
-        if e["totalBytes"] != e["groups"] * e["N"] * bb or e["offset"] + e["totalBytes"] > blob.size:
+        if e["kind"] == "i8":
+            want, extent = _int8_bytes(e), {"experts": e["experts"]}
+        else:
+            want, extent = e["groups"] * e["N"] * _block_bytes(e["kind"]), {"groups": e["groups"]}
+        if e["totalBytes"] != want or e["offset"] + e["totalBytes"] > blob.size:
             raise ValueError(f"loadQuantized: entry {e['name']} is inconsistent")
         buf = device.alloc(e["totalBytes"], device.PRIVATE)
         device.upload(buf, np.ascontiguousarray(blob[e["offset"]:e["offset"] + e["totalBytes"]]))
-        out[e["name"]] = (e["kind"], Quantized(buffer=buf, K=e["K"], N=e["N"], groups=e["groups"],
-                                               totalBytes=e["totalBytes"]))
+        out[e["name"]] = (e["kind"], Quantized(buffer=buf, K=e["K"], N=e["N"], totalBytes=e["totalBytes"], **extent))
     return out

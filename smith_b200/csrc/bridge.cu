@@ -53,11 +53,15 @@ enum KernelId {
   kMatmulQ4 = 0, kMatmulQ8 = 1, kQuantQ4 = 2, kQuantQ8 = 3,
   // the dense matmul family (shaders/matmul.metal): tiled, simple and batched, f32 and f16 storage
   kMatmulF32, kMatmulF16, kMatmulSimple, kMatmulSimpleF16, kMatmulBatched, kMatmulBatchedF16,
+  // the 8-bit integer products, f32 and f16 activations, and the sort that makes ragged groups
+  kQuantInt8, kQuantInt8F16, kMatmulInt8, kMatmulInt8F16, kMatmulInt8Grouped, kMatmulInt8GroupedF16, kGroupRows,
   kNumKernels
 };
 const char* const kKernelNames[kNumKernels] = {"matmul_q4", "matmul_q8", "quantize_q4", "quantize_q8",
                                                "matmul_f32", "matmul_f16", "matmul_simple", "matmul_simple_f16",
-                                               "matmul_batched", "matmul_batched_f16"};
+                                               "matmul_batched", "matmul_batched_f16", "quantize_int8", "quantize_int8_f16",
+                                               "matmul_int8", "matmul_int8_f16", "matmul_int8_grouped",
+                                               "matmul_int8_grouped_f16", "group_rows"};
 
 struct Context {
   uint32_t magic = kCtxMagic;
@@ -66,9 +70,17 @@ struct Context {
   cudaEvent_t base = nullptr;
   std::atomic<uint64_t> held{0};  // bytes held by live buffers + arenas
   uint64_t launches = 0;
-  void* stage[3] = {nullptr, nullptr, nullptr};
-  size_t stage_bytes[3] = {0, 0, 0};
+  void* stage[kMaxBind] = {nullptr};
+  size_t stage_bytes[kMaxBind] = {0};
   Workspace ws;
+  // Scratch of the int8 products.  A block that a captured graph refers to is not freed when a larger
+  // call needs more: it is kept aside until the context goes, so that the graph can still be replayed.
+  Workspace int8_ws;
+  bool int8_ws_captured = false;
+  struct Kept {
+    void* ptr;
+    Kept* next;
+  }* kept = nullptr;
   void* flush = nullptr;
   size_t flush_bytes = 0;
   bool capturing = false;
@@ -229,6 +241,84 @@ int output_ptr(Context* c, Buffer* b, int slot, size_t need, void** out, bool* c
 
 int ensure_workspace(Context* c, size_t need) { return grow(c, &c->ws.ptr, &c->ws.bytes, need); }
 
+int ensure_int8_workspace(Context* c, size_t need) {
+  if (c->int8_ws.bytes < need && c->int8_ws_captured) {
+    if (c->capturing) return fail("scratch memory must be sized before graph capture (need %zu bytes)", need);
+    Context::Kept* k = static_cast<Context::Kept*>(malloc(sizeof(Context::Kept)));
+    if (!k) return fail("out of host memory");
+    k->ptr = c->int8_ws.ptr, k->next = c->kept;
+    c->kept = k;
+    c->int8_ws = Workspace{};
+    c->int8_ws_captured = false;
+  }
+  if (grow(c, &c->int8_ws.ptr, &c->int8_ws.bytes, need)) return 1;
+  if (c->capturing) c->int8_ws_captured = true;
+  return 0;
+}
+
+bool overlap(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && a_bytes && b_bytes && x < y + b_bytes && y < x + a_bytes;
+}
+
+// Sizes the int8 kernels take; the message names the entry.
+int check_int8_sizes(const char* who, uint32_t dtype, uint64_t K, uint64_t N, uint64_t experts) {
+  if (dtype != kDenseF32 && dtype != kDenseF16) return fail("%s: dtype must be 0 (f32) or 1 (f16), got %u", who, dtype);
+  if (K < 1 || K > (uint64_t)kInt8MaxK)
+    return fail("%s: K = %llu is outside 1 .. %lld (the s32 sums)", who, (unsigned long long)K, (long long)kInt8MaxK);
+  if (N < 1 || N > (uint64_t)kInt8MaxN) return fail("%s: N = %llu is outside 1 .. %lld", who, (unsigned long long)N, (long long)kInt8MaxN);
+  if (experts < 1 || experts > (uint64_t)kInt8MaxExperts)
+    return fail("%s: %llu experts, 1 .. %lld are taken", who, (unsigned long long)experts, (long long)kInt8MaxExperts);
+  return 0;
+}
+
+int do_int8_pack(Context* c, uint32_t dtype, const void* w, void* out, uint64_t K, uint64_t N, uint64_t experts) {
+  if (reinterpret_cast<uintptr_t>(w) % (dtype == kDenseF16 ? 2 : 4)) return fail("int8_pack: the weights are not aligned to their type");
+  if (reinterpret_cast<uintptr_t>(out) & 15) return fail("int8_pack: the packed weights must start on 16 bytes");
+  cudaError_t e = launch_int8_pack((int)dtype, w, out, (int64_t)K, (int64_t)N, (int64_t)experts, c->stream);
+  return e == cudaSuccess ? 0 : fail("int8_pack launch failed: %s", cudaGetErrorString(e));
+}
+
+// Sizes are checked by the callers, addresses here.
+int do_int8_matmul(Context* c, const char* who, const Int8Gemm& g) {
+  const uint64_t es = g.dtype == kDenseF16 ? 2 : 4;
+  if (reinterpret_cast<uintptr_t>(g.A) % es || reinterpret_cast<uintptr_t>(g.C) % es)
+    return fail("%s: A and C must be aligned to their type", who);
+  if (reinterpret_cast<uintptr_t>(g.W) & 15) return fail("%s: the packed weights must start on 16 bytes", who);
+  for (const int* v : {g.offsets, g.position, g.order})
+    if (reinterpret_cast<uintptr_t>(v) & 3) return fail("%s: offsets, position and order must be aligned to 4 bytes", who);
+  const uint64_t c_bytes = ((uint64_t)(g.rows - 1) * g.ldc + g.N) * es;
+  if (overlap(g.C, c_bytes, g.W, int8_packed_bytes(g.K, g.N, g.experts)) ||
+      overlap(g.C, c_bytes, g.offsets, ((uint64_t)g.experts + 1) * 4) || overlap(g.C, c_bytes, g.order, (uint64_t)g.rows * 4))
+    return fail("%s: C overlaps the weights, the offsets or the order", who);
+  if (ensure_int8_workspace(c, int8_gemm_workspace_bytes(g.rows, g.K))) return 1;
+  cudaError_t e = launch_int8_gemm(g, c->int8_ws, c->stream);
+  return e == cudaSuccess ? 0 : fail("%s launch failed: %s", who, cudaGetErrorString(e));
+}
+
+int do_group_rows(Context* c, const int* ids, int* offsets, int* order, int* position, uint64_t rows, uint64_t experts) {
+  const void* out[3] = {offsets, order, position};
+  const uint64_t bytes[3] = {(experts + 1) * 4, rows * 4, rows * 4};
+  for (int i = 0; i < 3; i++) {
+    if (reinterpret_cast<uintptr_t>(out[i]) & 3) return fail("group_rows: buffers must be aligned to 4 bytes");
+    if (overlap(out[i], bytes[i], ids, rows * 4)) return fail("group_rows: an output overlaps the ids");
+    for (int j = 0; j < i; j++)
+      if (overlap(out[i], bytes[i], out[j], bytes[j])) return fail("group_rows: outputs overlap");
+  }
+  if (reinterpret_cast<uintptr_t>(ids) & 3) return fail("group_rows: buffers must be aligned to 4 bytes");
+  cudaError_t e = launch_group_rows(ids, (int64_t)rows, (int64_t)experts, offsets, order, position, c->stream);
+  return e == cudaSuccess ? 0 : fail("group_rows launch failed: %s", cudaGetErrorString(e));
+}
+
+constexpr uint64_t kMaxRows = 0x7FFFFFFFull - 1024;
+
+int check_group_rows(uint64_t rows, uint64_t experts) {
+  if (rows > kMaxRows) return fail("group_rows: %llu rows, at most %llu are taken", (unsigned long long)rows, (unsigned long long)kMaxRows);
+  if (experts < 1 || experts > (uint64_t)kInt8MaxExperts)
+    return fail("group_rows: %llu experts, 1 .. %lld are taken", (unsigned long long)experts, (long long)kInt8MaxExperts);
+  return 0;
+}
+
 int do_qmatmul(Context* c, int kind, const float* A, const uint8_t* B, float* C, uint64_t M, uint64_t N,
                uint64_t K, uint64_t groups, uint32_t path) {
   if (kind != 4 && kind != 8) return fail("kind must be 4 or 8, got %d", kind);
@@ -383,6 +473,103 @@ int submit(SmithEncoder* enc, cudaEvent_t e0, cudaEvent_t e1) {
       CU_TRY(cudaMemcpyAsync(enc->bufs[2]->host, cc, batch * M * N * es, cudaMemcpyDeviceToHost, c->stream));
     return 0;
   }
+  if (id == kQuantInt8 || id == kQuantInt8F16) {
+    const char* name = kKernelNames[id];
+    const uint32_t dtype = id == kQuantInt8F16 ? kDenseF16 : kDenseF32;
+    if (!enc->bufs[0] || !enc->bufs[1]) return fail("%s needs buffers 0 and 1", name);
+    if (enc->bytes[2].size() < 12) return fail("%s needs 12 bytes {K,N,experts} at index 2", name);
+    uint32_t prm[3];
+    memcpy(prm, enc->bytes[2].data(), 12);
+    const uint64_t K = prm[0], N = prm[1], E = prm[2], es = dtype == kDenseF16 ? 2 : 4;
+    if (check_int8_sizes(name, dtype, K, N, E)) return 1;
+    const void* w = nullptr;
+    void* o = nullptr;
+    bool back = false;
+    const size_t bytes = int8_packed_bytes((int64_t)K, (int64_t)N, (int64_t)E);
+    if (input_ptr(c, enc->bufs[0], 0, E * K * N * es, &w)) return 1;
+    if (output_ptr(c, enc->bufs[1], 1, bytes, &o, &back)) return 1;
+    if (e0) CU_TRY(cudaEventRecord(e0, c->stream));
+    if (do_int8_pack(c, dtype, w, o, K, N, E)) return 1;
+    if (e1) CU_TRY(cudaEventRecord(e1, c->stream));
+    if (back) CU_TRY(cudaMemcpyAsync(enc->bufs[1]->host, o, bytes, cudaMemcpyDeviceToHost, c->stream));
+    return 0;
+  }
+  if (id >= kMatmulInt8 && id <= kMatmulInt8GroupedF16) {
+    const char* name = kKernelNames[id];
+    const bool grouped = id >= kMatmulInt8Grouped;
+    const uint32_t dtype = (id == kMatmulInt8F16 || id == kMatmulInt8GroupedF16) ? kDenseF16 : kDenseF32;
+    const uint64_t es = dtype == kDenseF16 ? 2 : 4;
+    const size_t need = grouped ? 20 : 12;
+    for (int i = 0; i < 3; i++)
+      if (!enc->bufs[i]) return fail("%s needs buffers 0, 1 and 2", name);
+    if (grouped && !enc->bufs[4]) return fail("%s needs the offsets at index 4", name);
+    if (enc->bytes[3].size() < need)
+      return fail("%s needs %zu bytes %s at index 3", name, need, grouped ? "{rows,N,K,experts,fan}" : "{M,N,K}");
+    uint32_t prm[5] = {0, 0, 0, 1, 1};
+    memcpy(prm, enc->bytes[3].data(), need);
+    Int8Gemm g;
+    g.dtype = (int)dtype, g.rows = prm[0], g.N = prm[1], g.K = prm[2], g.experts = prm[3], g.lda = g.K, g.ldc = g.N;
+    if (check_int8_sizes(name, dtype, prm[2], prm[1], prm[3])) return 1;
+    if (prm[0] > kMaxRows) return fail("%s: too many rows (%u)", name, prm[0]);
+    uint64_t a_rows = prm[0];
+    if (grouped && enc->bufs[5]) {
+      if (prm[4] < 1 || prm[0] % prm[4]) return fail("%s: %u rows are no multiple of fan = %u", name, prm[0], prm[4]);
+      g.fan = (int)prm[4], a_rows = prm[0] / prm[4];
+    }
+    if (g.rows == 0) return 0;
+    const void* v = nullptr;
+    void* out = nullptr;
+    bool back = false;
+    const uint64_t c_bytes = (uint64_t)g.rows * g.N * es;
+    if (input_ptr(c, enc->bufs[0], 0, a_rows * g.K * es, &g.A)) return 1;
+    if (input_ptr(c, enc->bufs[1], 1, int8_packed_bytes(g.K, g.N, g.experts), &g.W)) return 1;
+    if (grouped) {
+      if (input_ptr(c, enc->bufs[4], 4, ((uint64_t)g.experts + 1) * 4, &v)) return 1;
+      g.offsets = static_cast<const int*>(v);
+      if (enc->bufs[5]) {
+        if (input_ptr(c, enc->bufs[5], 5, (uint64_t)g.rows * 4, &v)) return 1;
+        g.position = static_cast<const int*>(v);
+      }
+      if (enc->bufs[6]) {
+        if (input_ptr(c, enc->bufs[6], 6, (uint64_t)g.rows * 4, &v)) return 1;
+        g.order = static_cast<const int*>(v);
+      }
+    }
+    if (output_ptr(c, enc->bufs[2], 2, c_bytes, &out, &back)) return 1;
+    // rows of no expert keep what the caller's buffer holds, so a staged output starts from it
+    if (grouped && back) CU_TRY(cudaMemcpyAsync(out, enc->bufs[2]->host, c_bytes, cudaMemcpyHostToDevice, c->stream));
+    g.C = out;
+    if (e0) CU_TRY(cudaEventRecord(e0, c->stream));
+    if (do_int8_matmul(c, name, g)) return 1;
+    if (e1) CU_TRY(cudaEventRecord(e1, c->stream));
+    if (back) CU_TRY(cudaMemcpyAsync(enc->bufs[2]->host, out, c_bytes, cudaMemcpyDeviceToHost, c->stream));
+    return 0;
+  }
+  if (id == kGroupRows) {
+    for (int i = 0; i < 4; i++)
+      if (!enc->bufs[i]) return fail("group_rows needs buffers 0, 1, 2 and 3");
+    if (enc->bytes[4].size() < 8) return fail("group_rows needs 8 bytes {rows,experts} at index 4");
+    uint32_t prm[2];
+    memcpy(prm, enc->bytes[4].data(), 8);
+    const uint64_t rows = prm[0], E = prm[1];
+    if (check_group_rows(rows, E)) return 1;
+    const void* ids = nullptr;
+    void* out[3] = {nullptr};
+    bool back[3] = {false};
+    const uint64_t bytes[3] = {(E + 1) * 4, rows * 4, rows * 4};
+    if (input_ptr(c, enc->bufs[0], 0, rows * 4, &ids)) return 1;
+    for (int i = 0; i < 3; i++)
+      if (output_ptr(c, enc->bufs[i + 1], i + 1, bytes[i], &out[i], &back[i])) return 1;
+    if (e0) CU_TRY(cudaEventRecord(e0, c->stream));
+    if (do_group_rows(c, static_cast<const int*>(ids), static_cast<int*>(out[0]), static_cast<int*>(out[1]),
+                      static_cast<int*>(out[2]), rows, E))
+      return 1;
+    if (e1) CU_TRY(cudaEventRecord(e1, c->stream));
+    for (int i = 0; i < 3; i++)
+      if (back[i] && bytes[i])
+        CU_TRY(cudaMemcpyAsync(enc->bufs[i + 1]->host, out[i], bytes[i], cudaMemcpyDeviceToHost, c->stream));
+    return 0;
+  }
   if (id == kQuantQ4 || id == kQuantQ8) {
     const int kind = (id == kQuantQ4) ? 4 : 8;
     const size_t bb = (kind == 4) ? kQ4Bytes : kQ8Bytes;
@@ -420,9 +607,16 @@ void smith_destroy(void* p) {
   Context* c = as_ctx(p);
   if (!c) return;
   cudaStreamSynchronize(c->stream);
-  for (int i = 0; i < 3; i++)
+  for (int i = 0; i < kMaxBind; i++)
     if (c->stage[i]) cudaFree(c->stage[i]);
   if (c->ws.ptr) cudaFree(c->ws.ptr);
+  if (c->int8_ws.ptr) cudaFree(c->int8_ws.ptr);
+  while (c->kept) {
+    Context::Kept* k = c->kept;
+    c->kept = k->next;
+    cudaFree(k->ptr);
+    free(k);
+  }
   if (c->flush) cudaFree(c->flush);
   cudaEventDestroy(c->base);
   cudaStreamDestroy(c->stream);
@@ -885,6 +1079,88 @@ int32_t smith_qmatmul(void* p, uint32_t kind, void* a, void* b, void* cbuf, uint
   if (bc->bytes < M * N * 4) return fail("smith_qmatmul: C holds %llu bytes, needs %llu", (unsigned long long)bc->bytes,
                                          (unsigned long long)(M * N * 4));
   return do_qmatmul(c, (int)kind, (const float*)ba->dev, (const uint8_t*)bb->dev, (float*)bc->dev, M, N, K, groups, path);
+}
+
+uint64_t smith_int8_packed_bytes(uint64_t K, uint64_t N, uint64_t experts) {
+  if (check_int8_sizes("smith_int8_packed_bytes", kDenseF32, K, N, experts)) return 0;
+  return int8_packed_bytes((int64_t)K, (int64_t)N, (int64_t)experts);
+}
+
+int32_t smith_int8_pack(void* p, uint32_t dtype, void* w, void* out, uint64_t K, uint64_t N, uint64_t experts) {
+  Context* c = as_ctx(p);
+  Buffer *bw = as_buf(w), *bo = as_buf(out);
+  if (!c || !bw || !bo) return 1;
+  if (check_int8_sizes("smith_int8_pack", dtype, K, N, experts)) return 1;
+  if (!bw->dev || !bo->dev) return fail("smith_int8_pack needs buffers with a device side");
+  const uint64_t in = experts * K * N * (dtype == kDenseF16 ? 2 : 4), need = int8_packed_bytes(K, N, experts);
+  if (bw->bytes < in || bo->bytes < need)
+    return fail("smith_int8_pack: buffers of %llu and %llu bytes, needs %llu and %llu", (unsigned long long)bw->bytes,
+                (unsigned long long)bo->bytes, (unsigned long long)in, (unsigned long long)need);
+  if (overlap(bw->dev, in, bo->dev, need)) return fail("smith_int8_pack: the packed weights overlap the weights");
+  return do_int8_pack(c, dtype, bw->dev, bo->dev, K, N, experts);
+}
+
+int32_t smith_int8_matmul(void* p, uint32_t dtype, void* a, void* w, void* cbuf, uint64_t M, uint64_t N, uint64_t K,
+                          uint64_t lda, uint64_t ldc) {
+  return smith_int8_matmul_grouped(p, dtype, a, w, nullptr, cbuf, M, N, K, 1, lda, ldc, nullptr, nullptr, 1);
+}
+
+int32_t smith_int8_matmul_grouped(void* p, uint32_t dtype, void* a, void* w, void* offsets, void* cbuf, uint64_t rows,
+                                  uint64_t N, uint64_t K, uint64_t experts, uint64_t lda, uint64_t ldc, void* position,
+                                  void* order, uint64_t fan) {
+  Context* c = as_ctx(p);
+  Buffer *ba = as_buf(a), *bw = as_buf(w), *bc = as_buf(cbuf);
+  if (!c || !ba || !bw || !bc) return 1;
+  const char* who = offsets || experts != 1 ? "smith_int8_matmul_grouped" : "smith_int8_matmul";
+  if (check_int8_sizes(who, dtype, K, N, experts)) return 1;
+  if (rows > kMaxRows) return fail("%s: %llu rows, at most %llu are taken", who, (unsigned long long)rows, (unsigned long long)kMaxRows);
+  if (!ba->dev || !bw->dev || !bc->dev) return fail("%s needs buffers with a device side", who);
+  if (!lda) lda = K;
+  if (!ldc) ldc = N;
+  if (lda < K || ldc < N || lda > 0x7FFFFFFFull || ldc > 0x7FFFFFFFull)
+    return fail("%s: row pitches lda = %llu, ldc = %llu do not fit K = %llu, N = %llu", who, (unsigned long long)lda,
+                (unsigned long long)ldc, (unsigned long long)K, (unsigned long long)N);
+  if (!offsets && (experts != 1 || position || order)) return fail("%s: experts, position and order need offsets", who);
+  if (!position && fan != 1) return fail("%s: fan = %llu needs a position list", who, (unsigned long long)fan);
+  if (fan < 1 || rows % fan) return fail("%s: %llu rows are no multiple of fan = %llu", who, (unsigned long long)rows, (unsigned long long)fan);
+  if (rows == 0) return 0;
+  Int8Gemm g;
+  g.dtype = (int)dtype, g.A = ba->dev, g.lda = (int64_t)lda, g.W = bw->dev, g.C = bc->dev, g.ldc = (int64_t)ldc;
+  g.rows = (int64_t)rows, g.N = (int64_t)N, g.K = (int64_t)K, g.experts = (int64_t)experts, g.fan = (int)fan;
+  const uint64_t es = dtype == kDenseF16 ? 2 : 4;
+  const uint64_t a_need = ((rows / fan - 1) * lda + K) * es, c_need = ((rows - 1) * ldc + N) * es;
+  if (ba->bytes < a_need) return fail("%s: A holds %llu bytes, needs %llu", who, (unsigned long long)ba->bytes, (unsigned long long)a_need);
+  if (bc->bytes < c_need) return fail("%s: C holds %llu bytes, needs %llu", who, (unsigned long long)bc->bytes, (unsigned long long)c_need);
+  const uint64_t w_need = int8_packed_bytes(K, N, experts);
+  if (bw->bytes < w_need)
+    return fail("%s: the packed weights hold %llu bytes, needs %llu", who, (unsigned long long)bw->bytes, (unsigned long long)w_need);
+  struct List { void* buf; uint64_t count; const int** at; const char* name; };
+  for (const List& l : {List{offsets, experts + 1, &g.offsets, "offsets"}, List{position, rows, &g.position, "position"},
+                        List{order, rows, &g.order, "order"}}) {
+    if (!l.buf) continue;
+    Buffer* b = as_buf(l.buf);
+    if (!b) return 1;
+    if (!b->dev) return fail("%s needs buffers with a device side", who);
+    if (b->bytes < l.count * 4)
+      return fail("%s: %s holds %llu bytes, needs %llu", who, l.name, (unsigned long long)b->bytes, (unsigned long long)(l.count * 4));
+    *l.at = static_cast<const int*>(b->dev);
+  }
+  return do_int8_matmul(c, who, g);
+}
+
+int32_t smith_group_rows(void* p, void* ids, void* offsets, void* order, void* position, uint64_t rows, uint64_t experts) {
+  Context* c = as_ctx(p);
+  Buffer* b[4] = {as_buf(ids), as_buf(offsets), as_buf(order), as_buf(position)};
+  if (!c || !b[0] || !b[1] || !b[2] || !b[3]) return 1;
+  if (check_group_rows(rows, experts)) return 1;
+  const uint64_t need[4] = {rows * 4, (experts + 1) * 4, rows * 4, rows * 4};
+  for (int i = 0; i < 4; i++) {
+    if (!b[i]->dev) return fail("smith_group_rows needs buffers with a device side");
+    if (b[i]->bytes < need[i])
+      return fail("smith_group_rows: buffer %d holds %llu bytes, needs %llu", i, (unsigned long long)b[i]->bytes, (unsigned long long)need[i]);
+  }
+  return do_group_rows(c, static_cast<const int*>(b[0]->dev), static_cast<int*>(b[1]->dev), static_cast<int*>(b[2]->dev),
+                       static_cast<int*>(b[3]->dev), rows, experts);
 }
 
 int32_t smith_matmul(void* p, uint32_t dtype, void* a, void* b, void* cbuf, uint64_t M, uint64_t N, uint64_t K,

@@ -147,6 +147,33 @@ uint64_t qgemv_list_weight_bytes(const ListProgram* lp);
 cudaError_t launch_qgemm_tc_static(int kind, const float* A, const uint8_t* B, float* C, int64_t M, int64_t N,
                                    int64_t K, int64_t groups, cudaStream_t s, const char** why);
 
+// int8_rows.cu / int8_gemm.cu : the W8A8 product.  Weights [experts][K][N] f32 or f16 are packed once; a
+// product quantises its activations per row into scratch and multiplies on the integer tensor cores.
+constexpr int64_t kInt8MaxK = 131072;        // 127^2 * K stays below 2^31
+constexpr int64_t kInt8MaxN = 1 << 22;       // channel tiles of 128 stay below 2^16
+constexpr int64_t kInt8MaxExperts = 1024;
+size_t int8_packed_bytes(int64_t K, int64_t N, int64_t experts);
+cudaError_t launch_int8_pack(int dtype, const void* w, void* out, int64_t K, int64_t N, int64_t experts, cudaStream_t s);
+struct Int8Gemm {
+  int dtype = 0;                 // of A and C: kDenseF32 or kDenseF16
+  const void* A = nullptr;       // [rows][K] (with position: [rows / fan][K]), pitch lda elements
+  int64_t lda = 0;
+  const void* W = nullptr;       // packed
+  void* C = nullptr;             // [rows][N], pitch ldc elements
+  int64_t ldc = 0;
+  int64_t rows = 0, N = 0, K = 0, experts = 1;
+  const int* offsets = nullptr;  // null: all rows meet the one matrix; else [experts + 1], rows sorted by expert
+  const int* position = nullptr; // null, or [rows]: row t of A goes to sorted places position[t * fan ..]
+  int fan = 1;
+  const int* order = nullptr;    // null, or [rows]: sorted row j is row order[j] of C
+};
+size_t int8_gemm_workspace_bytes(int64_t rows, int64_t K);
+cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s);
+
+// group_rows.cu : stable counting sort of rows by expert id.
+cudaError_t launch_group_rows(const int* ids, int64_t rows, int64_t experts, int* offsets, int* order, int* position,
+                              cudaStream_t s);
+
 // util.cu
 // Number of SMs of the current device (cached per device; 148 if the query fails).
 int device_sm_count();

@@ -65,6 +65,37 @@ __device__ __forceinline__ void umma_f16_kblock(uint32_t d_tmem, uint32_t a_lo, 
       "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
       : "memory");
 }
+// The same for 8-bit integers (D s32): the 128-byte row is 128 values of k, four MMAs 128 x N x 32.
+__device__ __forceinline__ void umma_i8_kblock(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi,
+                                               uint32_t idesc, uint32_t accumulate_first) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      ".reg .b32 ta, tb;\n"
+      ".reg .b64 da, db;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "setp.ne.b32 q, %4, 0;\n"
+      "mov.b64 da, {%1, %3};\n"
+      "mov.b64 db, {%2, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, p;\n"
+      "add.u32 ta, %1, 2;\n"
+      "add.u32 tb, %2, 2;\n"
+      "mov.b64 da, {ta, %3};\n"
+      "mov.b64 db, {tb, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
+      "add.u32 ta, %1, 4;\n"
+      "add.u32 tb, %2, 4;\n"
+      "mov.b64 da, {ta, %3};\n"
+      "mov.b64 db, {tb, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
+      "add.u32 ta, %1, 6;\n"
+      "add.u32 tb, %2, 6;\n"
+      "mov.b64 da, {ta, %3};\n"
+      "mov.b64 db, {tb, %3};\n"
+      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
+      "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
+      : "memory");
+}
 // mbarrier arrive once every MMA issued so far by this thread has completed.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");

@@ -97,6 +97,11 @@ SYMBOLS = {
     "smith_gguf_repack": (_i32, [_p, _u32, _p, _p, _u64, _u64]),
     "smith_qmatmul": (_i32, [_p, _u32, _p, _p, _p, _u64, _u64, _u64, _u64, _u32]),
     "smith_matmul": (_i32, [_p, _u32, _p, _p, _p, _u64, _u64, _u64, _u64, _u32]),
+    "smith_int8_packed_bytes": (_u64, [_u64, _u64, _u64]),
+    "smith_int8_pack": (_i32, [_p, _u32, _p, _p, _u64, _u64, _u64]),
+    "smith_int8_matmul": (_i32, [_p, _u32, _p, _p, _p, _u64, _u64, _u64, _u64, _u64]),
+    "smith_int8_matmul_grouped": (_i32, [_p, _u32, _p, _p, _p, _p, _u64, _u64, _u64, _u64, _u64, _u64, _p, _p, _u64]),
+    "smith_group_rows": (_i32, [_p, _p, _p, _p, _p, _u64, _u64]),
     "smith_qmatmul_path": (_i32, [_u32, _u64, _u64, _u64]),
     "smith_qmatmul_list_create": (_p, [_p, _u32, _u64, C.POINTER(SmithListItem), _u32]),
     "smith_qmatmul_list_create_gather": (_p, [_p, _u32, _u64, C.POINTER(SmithListItem), C.POINTER(SmithListGather), _u32, _u32,
@@ -443,6 +448,40 @@ DENSE_AUTO, DENSE_GENERIC, DENSE_TENSOR, DENSE_TENSOR_FAST = 0, 1, 2, 3
 def matmul(dtype, aBuffer, bBuffer, cBuffer, M, N, K, batch=1, path=DENSE_AUTO):
     """smith_matmul: the dense matmul c[batch,M,N] = a[batch,M,K] @ b[batch,K,N] on device-side buffers."""
     _check(lib.smith_matmul(ctx(), dtype, aBuffer, bBuffer, cBuffer, M, N, K, batch, path), "matmul")
+
+
+def int8PackedBytes(K, N, experts=1):
+    """Bytes of the packed weights [experts][K][N] of the int8 products."""
+    n = int(lib.smith_int8_packed_bytes(K, N, experts))
+    if not n:
+        _raise("int8_packed_bytes")
+    return n
+
+
+def int8Pack(dtype, wBuffer, outBuffer, K, N, experts=1):
+    _check(lib.smith_int8_pack(ctx(), dtype, wBuffer, outBuffer, K, N, experts), "int8_pack")
+
+
+def int8Matmul(dtype, aBuffer, wBuffer, cBuffer, M, N, K, lda=0, ldc=0):
+    """smith_int8_matmul: c[M,N] = a[M,K] x packed w, codes of a made per row; asynchronous."""
+    if lib.smith_int8_matmul(ctx(), dtype, aBuffer, wBuffer, cBuffer, M, N, K, lda, ldc):
+        _raise("int8_matmul")
+
+
+def int8MatmulGrouped(dtype, aBuffer, wBuffer, offsetsBuffer, cBuffer, rows, N, K, experts, lda=0, ldc=0,
+                      positionBuffer=None, orderBuffer=None, fan=1):
+    """smith_int8_matmul_grouped: rows sorted by expert, a matrix per expert (see the header); asynchronous."""
+    if not offsetsBuffer:
+        raise SmithError("smith: int8_matmul_grouped: the offsets are missing")
+    if lib.smith_int8_matmul_grouped(ctx(), dtype, aBuffer, wBuffer, offsetsBuffer, cBuffer, rows, N, K, experts, lda,
+                                     ldc, positionBuffer, orderBuffer, fan):
+        _raise("int8_matmul_grouped")
+
+
+def groupRows(idsBuffer, offsetsBuffer, orderBuffer, positionBuffer, rows, experts):
+    """smith_group_rows: the lists of a ragged product from the rows' expert ids; asynchronous."""
+    if lib.smith_group_rows(ctx(), idsBuffer, offsetsBuffer, orderBuffer, positionBuffer, rows, experts):
+        _raise("group_rows")
 
 
 def qmatmulStatic(kind, aPtr, bPtr, cPtr, M, N, K, groups, streamPtr=None):

@@ -38,7 +38,10 @@ def setPeaks(hbmGBs=None, tensorTFlops=None, source="caller"):
 def algorithmicCost(kernelName, params):
     """(bytes, flops) of one dispatch of a kernel from its parameter block, else None.
     matmul_q4 / matmul_q8: params = [M, N, K, groups]; quantize_q4 / quantize_q8: params = [K, N];
-    matmul_f32 / matmul_f16 / matmul_simple[_f16] / matmul_batched[_f16]: params = [M, N, K(, batch)]."""
+    matmul_f32 / matmul_f16 / matmul_simple[_f16] / matmul_batched[_f16]: params = [M, N, K(, batch)];
+    quantize_int8[_f16]: params = [K, N, experts]; matmul_int8[_f16]: params = [M, N, K];
+    matmul_int8_grouped[_f16]: params = [rows, N, K, experts, fan], where how many experts hold a row is on
+    the device: at most min(rows, experts) are counted; group_rows: params = [rows, experts]."""
     if params is None:
         return None
     p = [int(v) for v in params]
@@ -50,6 +53,16 @@ def algorithmicCost(kernelName, params):
         K, N = p[:2]
         bb = 24 if kernelName == "quantize_q4" else 34
         return 4 * K * N + ((K + 31) // 32) * N * bb, 0
+    if kernelName in ("quantize_int8", "quantize_int8_f16") and len(p) >= 3:
+        K, N, experts = p[:3]
+        return experts * N * ((2 if kernelName.endswith("_f16") else 4) * K + K + 4), 0
+    if kernelName in ("matmul_int8", "matmul_int8_f16", "matmul_int8_grouped", "matmul_int8_grouped_f16") and len(p) >= 3:
+        M, N, K = p[:3]
+        experts, fan = (p[3], p[4]) if "grouped" in kernelName and len(p) >= 5 else (1, 1)
+        es = 2 if kernelName.endswith("_f16") else 4
+        return es * (M // fan * K + M * N) + min(M, experts) * N * (K + 4), 2 * M * K * N
+    if kernelName == "group_rows" and len(p) >= 2:
+        return 4 * (3 * p[0] + p[1] + 1), 0
     if kernelName.startswith("matmul_") and len(p) >= 3:
         # the dense family: [M, N, K] or [M, N, K, batch]; f16 storage in the names that end in _f16
         M, N, K = p[:3]

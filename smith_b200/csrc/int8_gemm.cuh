@@ -16,7 +16,9 @@ int8_layout int8_weight_layout(int64_t K, int64_t N, int64_t experts);
 // Codes and maxima (NaN for a row that is not finite) of `rows` rows of a [rows][K] (pitch lda elements; dtype kDenseF32 / kDenseF16):
 // codes [places][K rounded up to 128] and maxima [places]; row r goes to place r, or with `position` to
 // the places position[r * fan .. r * fan + fan).  Places outside [0, places) are skipped.
+// n_counters words at `counters` are set to 0.
 cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda, int64_t K, const int* position, int fan,
-                             int64_t places, uint8_t* codes, float* maxima, cudaStream_t s);
+                             int64_t places, uint8_t* codes, float* maxima, int* counters, int n_counters,
+                             cudaStream_t s);
 
 }  // namespace smith

@@ -102,11 +102,14 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const T* __restrict__ w,
 template <typename T>
 __global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ a, int64_t lda, int64_t K, int64_t kp,
                                                         const int* __restrict__ position, int fan, int64_t places,
-                                                        uint8_t* __restrict__ codes, float* __restrict__ maxima) {
+                                                        uint8_t* __restrict__ codes, float* __restrict__ maxima, int* __restrict__ counters,
+                                                        int n_counters) {
   // Wait first, then let the product start: what precedes this launch is finished by then, so the
   // product may read weights and group boundaries before its own wait.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (blockIdx.x == 0)                       // the product's counters of shared tiles start at 0 in every call
+    for (int i = threadIdx.x; i < n_counters; i += 256) counters[i] = 0;
   __shared__ unsigned warp_most[8];
   const int64_t row = blockIdx.x;
   const T* x = a + row * lda;
@@ -171,7 +174,8 @@ cudaError_t launch_int8_pack(int dtype, const void* w, void* out, int64_t K, int
 }
 
 cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda, int64_t K, const int* position, int fan,
-                             int64_t places, uint8_t* codes, float* maxima, cudaStream_t s) {
+                             int64_t places, uint8_t* codes, float* maxima, int* counters, int n_counters,
+                             cudaStream_t s) {
   const int64_t kp = (K + 127) / 128 * 128;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -181,8 +185,10 @@ cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda
   cfg.attrs = &attr, cfg.numAttrs = 1;
   count_launch();
   if (dtype == kDenseF16)
-    return cudaLaunchKernelEx(&cfg, int8_rows_kernel<__half>, (const __half*)a, lda, K, kp, position, fan, places, codes, maxima);
-  return cudaLaunchKernelEx(&cfg, int8_rows_kernel<float>, (const float*)a, lda, K, kp, position, fan, places, codes, maxima);
+    return cudaLaunchKernelEx(&cfg, int8_rows_kernel<__half>, (const __half*)a, lda, K, kp, position, fan, places, codes, maxima,
+                              counters, n_counters);
+  return cudaLaunchKernelEx(&cfg, int8_rows_kernel<float>, (const float*)a, lda, K, kp, position, fan, places, codes, maxima, counters,
+                            n_counters);
 }
 
 }  // namespace smith

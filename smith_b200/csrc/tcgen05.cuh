@@ -65,7 +65,7 @@ __device__ __forceinline__ void umma_f16_kblock(uint32_t d_tmem, uint32_t a_lo, 
       "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
       : "memory");
 }
-// The same for 8-bit integers (D s32): the 128-byte row is 128 values of k, four MMAs 128 x N x 32.
+// The four MMAs of one 128-byte slab of 8-bit integers (D s32): 128 k, 128 x N x 32 each.
 __device__ __forceinline__ void umma_i8_kblock(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi,
                                                uint32_t idesc, uint32_t accumulate_first) {
   asm volatile(
@@ -152,6 +152,9 @@ __device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t caddr) {
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(caddr) : "memory");
   return v;
 }
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t cbar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cbar) : "memory");
+}
 __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t cbar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cbar), "r"(bytes) : "memory");
 }
@@ -199,6 +202,37 @@ __device__ __forceinline__ void umma_f16_kblock_pair(uint32_t d_tmem, uint32_t a
       "mov.b64 da, {ta, %3};\n"
       "mov.b64 db, {tb, %3};\n"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, q;\n"
+      "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
+      : "memory");
+}
+// The four MMAs of one 128-byte slab of 8-bit integers (D s32): 256 x N x 32 each, on a CTA pair.
+__device__ __forceinline__ void umma_i8_kblock_pair(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi,
+                                               uint32_t idesc, uint32_t accumulate_first) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      ".reg .b32 ta, tb;\n"
+      ".reg .b64 da, db;\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "setp.ne.b32 q, %4, 0;\n"
+      "mov.b64 da, {%1, %3};\n"
+      "mov.b64 db, {%2, %3};\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, p;\n"
+      "add.u32 ta, %1, 2;\n"
+      "add.u32 tb, %2, 2;\n"
+      "mov.b64 da, {ta, %3};\n"
+      "mov.b64 db, {tb, %3};\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
+      "add.u32 ta, %1, 4;\n"
+      "add.u32 tb, %2, 4;\n"
+      "mov.b64 da, {ta, %3};\n"
+      "mov.b64 db, {tb, %3};\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
+      "add.u32 ta, %1, 6;\n"
+      "add.u32 tb, %2, 6;\n"
+      "mov.b64 da, {ta, %3};\n"
+      "mov.b64 db, {tb, %3};\n"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
       "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
       : "memory");
 }

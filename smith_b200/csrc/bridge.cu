@@ -291,7 +291,7 @@ int do_int8_matmul(Context* c, const char* who, const Int8Gemm& g) {
   if (overlap(g.C, c_bytes, g.W, int8_packed_bytes(g.K, g.N, g.experts)) ||
       overlap(g.C, c_bytes, g.offsets, ((uint64_t)g.experts + 1) * 4) || overlap(g.C, c_bytes, g.order, (uint64_t)g.rows * 4))
     return fail("%s: C overlaps the weights, the offsets or the order", who);
-  if (ensure_int8_workspace(c, int8_gemm_workspace_bytes(g.rows, g.K, g.experts, g.offsets != nullptr))) return 1;
+  if (ensure_int8_workspace(c, int8_gemm_workspace_bytes(g.rows, g.N, g.K, g.experts, g.offsets != nullptr))) return 1;
   cudaError_t e = launch_int8_gemm(g, c->int8_ws, c->stream);
   return e == cudaSuccess ? 0 : fail("%s launch failed: %s", who, cudaGetErrorString(e));
 }

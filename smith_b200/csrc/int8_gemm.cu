@@ -21,11 +21,12 @@
 //
 //   warp 0     producer: one copy of the packed 16 KB weight block and one box of token codes per unit
 //   warp 1     MMA issuer; two accumulators in tensor memory, so the next tile runs during an epilogue
-//   warps 2-5  epilogue
+//   warps 2-9  epilogue: two warps share a quarter of the lanes and take its 32-token chunks in turn
 // Every mbarrier wait is time-bounded (pipeline.cuh); on a give-up the CTA waits (bounded) for its copies
 // and MMAs in flight, frees its tensor memory and leaves the status word set.
 #include <cuda.h>
 #include <cuda_fp16.h>
+#include <math.h>
 
 #include "int8_gemm.cuh"
 #include "kernels.h"
@@ -36,12 +37,14 @@
 namespace smith {
 namespace {
 
-constexpr int kThreads = 6 * 32;
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr int kWTile = 16384;         // 128 channels x 128 k
 constexpr int kMaxStages = 12;
-constexpr int kHeader = 1536;         // barriers; the group lists follow
-constexpr int kSplitCost = 8;         // units of time that joining a shared tile costs (see `share` below)
-constexpr int kMinUnits = 4;          // fewest units per worker
+constexpr int kHeader = 2560;         // barriers; the group lists follow
+constexpr int kMinUnits = 2;          // fewest units per worker
+constexpr int kMaxPieces = 16;        // most pieces per tile
+constexpr int kBlock = 8;             // token tiles side by side
 
 struct Params {
   const uint8_t* w;
@@ -50,11 +53,13 @@ struct Params {
   const int* offsets;                 // null: one group of all rows; else [experts + 1]
   const int* order;                   // null, or the row of C for each sorted row
   void* C;
-  int* partial;                       // two slots of [BT][128] per CTA
-  int* counters;                      // four per CTA, one for each epilogue warp
+  int4* partial;                      // two slots of [BT / 4][128] per CTA
+  int* counters;                      // one per epilogue warp of each CTA
+  float join_fixed, join_each;        // what joining a shared tile costs, in units: once, and per worker joined
   int64_t ldc;
   int rows, N, experts;
   int n_tiles, k_slabs;
+  int w_tiles;                        // n_tiles, in pairs for the pair form
   int BT;                             // tokens per tile
   int workers;
   int stages, stage_bytes, header, tmem_cols;
@@ -75,8 +80,9 @@ __device__ __noinline__ float scaled(int sum, float sa, float sw, float a_max, f
   return (float)((double)sum * ((double)a_max / 127.0) * ((double)w_max / 127.0));
 }
 
-__device__ __forceinline__ void put(float* at, float v) { *at = v; }
-__device__ __forceinline__ void put(__half* at, float v) { *at = __float2half_rn(v); }
+// C is written once and not read here: it should not push weights and codes out of L2
+__device__ __forceinline__ void put(float* at, float v) { __stcs(at, v); }
+__device__ __forceinline__ void put(__half* at, float v) { __stcs(at, __float2half_rn(v)); }
 
 // Up to 32 tokens of one channel: sums r scaled and stored; sa and to (row of C, negative: none) are the
 // chunk's in shared memory.  `first` is the chunk's first row of C where rows are in order.
@@ -104,6 +110,19 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], int count, 
   }
 }
 
+// The same for a chunk with a scale outside the plain range; rare, so kept out of line.
+__device__ __noinline__ void store_odd(const Params& p, const uint32_t (&r)[32], const float* sa, const int* to, float sw, float a_max,
+                                       float w_max, int n, bool mine) {
+#pragma unroll
+  for (int i = 0; i < 32; i++) {
+    const float v = scaled((int)r[i], sa[i], sw, __shfl_sync(0xffffffffu, a_max, i), w_max);
+    if (to[i] >= 0 && mine) {
+      if (p.out_f16) put(static_cast<__half*>(p.C) + to[i] * p.ldc + n, v);
+      else put(static_cast<float*>(p.C) + to[i] * p.ldc + n, v);
+    }
+  }
+}
+
 // ---------------------------------------------------------------- the schedule
 // Equal contiguous runs of `total` units over `workers`: the first total % workers runs hold one more.
 struct Deal {
@@ -116,36 +135,62 @@ struct Deal {
   }
 };
 
+// A worker's work: tile i * workers + worker of each full wave, then its run of the units of what is left.
 struct Schedule {
   const int* row_first;     // [experts + 1] cleaned group boundaries
   const int* tile_first;    // [experts + 1] first tile of each group
-  int64_t unit0, unit1;     // this worker's run
-  Deal deal;                // of units, or of whole tiles
-  int k_slabs;
-  bool share;               // tiles may be shared
+  int worker, waves;
+  int64_t shared0;          // first tile that may be shared
+  Deal deal;                // units from there on
+  int64_t u, end;           // this worker's run of them
 };
 
-struct Tile {
+struct Segment {            // slabs [ks0, ks1) of a tile
   int expert, nt, row0, rows;
+  int ks0, ks1;
+  int64_t unit;             // of the tile's slab 0, counted from shared0
 };
 
-// Tile t (the cursor e only moves forward).
-__device__ __forceinline__ Tile tile_at(const Params& p, const Schedule& s, int64_t t, int& e) {
-  while (t >= s.tile_first[e + 1]) e++;
-  const int first = s.row_first[e], count = s.row_first[e + 1] - first;
-  const int tt = (count + p.BT - 1) / p.BT;
-  const int x = (int)t - s.tile_first[e];
-  const int mt = x % tt;
-  return {e, x / tt, first + mt * p.BT, min(count - mt * p.BT, p.BT)};
-}
+struct Walk {
+  int wave = 0, e = 0;      // tiles only rise, so the group cursor only moves forward
+  int64_t u;
+  __device__ explicit Walk(const Schedule& s) : u(s.u) {}
+  __device__ __forceinline__ bool next(const Params& p, const Schedule& s, Segment& g) {
+    int64_t t;
+    if (wave < s.waves) {
+      t = (int64_t)wave * p.workers + s.worker;
+      wave++;
+      g.ks0 = 0, g.ks1 = p.k_slabs, g.unit = 0;
+    } else {
+      if (u >= s.end) return false;
+      t = u / p.k_slabs;
+      g.unit = t * p.k_slabs;
+      g.ks0 = (int)(u - g.unit), g.ks1 = (int)min((int64_t)p.k_slabs, s.end - g.unit);
+      u = g.unit + g.ks1;
+      t += s.shared0;
+    }
+    while (t >= s.tile_first[e + 1]) e++;
+    const int first = s.row_first[e], count = s.row_first[e + 1] - first;
+    const int w_tiles = p.w_tiles;
+    // blocks of up to kBlock token tiles by all weight tiles, tokens fastest: what runs at one time is
+    // compact, so the codes of both sides are fetched by many workers at once
+    const int tt = (count + p.BT - 1) / p.BT, x = (int)t - s.tile_first[e];
+    const int block = x / (kBlock * w_tiles), in_block = x - block * (kBlock * w_tiles);
+    const int width = min(kBlock, tt - block * kBlock);
+    g.nt = in_block / width;
+    const int mt = block * kBlock + in_block - g.nt * width;
+    g.expert = e, g.row0 = first + mt * p.BT, g.rows = min(count - mt * p.BT, p.BT);
+    return true;
+  }
+};
 
 // Group boundaries come from device memory: clamped and made to rise, so that nothing they hold leads
 // outside the rows or covers a row twice.  One warp; tiles of a group = weight tiles x token tiles.
-__device__ __forceinline__ void plan_groups(const Params& p, int w_tiles, int* row_first, int* tile_first, int lane) {
+__device__ __forceinline__ void plan_groups(const Params& p, int* row_first, int* tile_first, int lane) {
   int high = 0, tiles = 0;
   if (lane == 0) tile_first[0] = 0;
   if (!p.offsets) {
-    if (lane == 0) row_first[0] = 0, row_first[1] = p.rows, tile_first[1] = w_tiles * ((p.rows + p.BT - 1) / p.BT);
+    if (lane == 0) row_first[0] = 0, row_first[1] = p.rows, tile_first[1] = p.w_tiles * ((p.rows + p.BT - 1) / p.BT);
     return;
   }
   for (int i0 = 0; i0 <= p.experts; i0 += 32) {
@@ -156,7 +201,7 @@ __device__ __forceinline__ void plan_groups(const Params& p, int w_tiles, int* r
     int before = __shfl_up_sync(0xffffffffu, v, 1);
     if (lane == 0) before = high;                       // boundary i - 1
     high = __shfl_sync(0xffffffffu, v, 31);
-    int t = (i >= 1 && i <= p.experts) ? w_tiles * ((v - before + p.BT - 1) / p.BT) : 0;
+    int t = (i >= 1 && i <= p.experts) ? p.w_tiles * ((v - before + p.BT - 1) / p.BT) : 0;
     for (int d = 1; d < 32; d <<= 1) {
       const int u = __shfl_up_sync(0xffffffffu, t, d);
       if (lane >= d) t += u;
@@ -167,9 +212,38 @@ __device__ __forceinline__ void plan_groups(const Params& p, int w_tiles, int* r
   }
 }
 
+// Token c of a tile: its maximum and its row of C (-1: none).
+__device__ __forceinline__ void fetch_token(const Params& p, const Segment& tile, int c, float& a_max, int& to) {
+  a_max = 0.f, to = -1;
+  if (c < tile.rows) {
+    const int row = tile.row0 + c;
+    a_max = p.a_max[row];
+    to = p.order ? p.order[row] : row;
+    if (to >= p.rows) to = -1;
+  }
+}
+
+// Adds the partial sums of a tile's other workers to one chunk.
+__device__ __forceinline__ void join(const Params& p, const Segment& tile, uint32_t (&r)[32], int c, int ctas, int rank, int worker, int w0,
+                                     int others, int ch) {
+#pragma unroll 2
+  for (int k = 0; k < others; k++) {
+    const int w = w0 + k + (w0 + k >= worker ? 1 : 0);
+    const int4* slot = p.partial + ((size_t)(ctas * w + rank) * 2 + (w == w0 ? 1 : 0)) * (p.BT * 32) + (c >> 2) * 128 + ch;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (c + 4 * i < tile.rows) {
+        const int4 v = __ldcg(&slot[i * 128]);
+        r[4 * i] += (uint32_t)v.x, r[4 * i + 1] += (uint32_t)v.y, r[4 * i + 2] += (uint32_t)v.z, r[4 * i + 3] += (uint32_t)v.w;
+      }
+    }
+  }
+}
+
 template <bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
-                                                                const __grid_constant__ CUtensorMap tmap_w, const Params p) {
+                                                                const __grid_constant__ CUtensorMap tmap_w,
+                                                                const __grid_constant__ Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);     // [kMaxStages] a stage's codes landed
   uint64_t* empty = full + kMaxStages;                     // [kMaxStages] its MMAs are done
@@ -178,24 +252,23 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
   uint64_t* drain = acc_empty + 2;                         // [1] MMAs in flight, after a give-up
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* chunk_sa = reinterpret_cast<float*>(smem + 320) + ((threadIdx.x >> 5) & 3) * 32;   // [4][32] per epilogue warp
-  int* chunk_to = reinterpret_cast<int*>(smem + 320 + 512) + ((threadIdx.x >> 5) & 3) * 32;
+  float* chunk_sa = reinterpret_cast<float*>(smem + 512) + ((threadIdx.x >> 5) & 7) * 32;   // [8][32] per epilogue warp
+  int* chunk_to = reinterpret_cast<int*>(smem + 512 + 1024) + ((threadIdx.x >> 5) & 7) * 32;
   int* row_first = reinterpret_cast<int*>(smem + kHeader);
   int* tile_first = row_first + p.experts + 1;
   uint8_t* tiles = smem + p.header;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;    // 0: the CTA that issues the pair's MMAs
   const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x;
-  const int w_tiles = PAIR ? (p.n_tiles + 1) / 2 : p.n_tiles;
 
   if (tid == 0) {
     for (int s = 0; s < kMaxStages; s++) mbar_init(smem_u32(&full[s]), PAIR ? 2 : 1), mbar_init(smem_u32(&empty[s]), 1);
-    for (int b = 0; b < 2; b++) mbar_init(smem_u32(&acc_full[b]), 1), mbar_init(smem_u32(&acc_empty[b]), PAIR ? 8 : 4);
+    for (int b = 0; b < 2; b++) mbar_init(smem_u32(&acc_full[b]), 1), mbar_init(smem_u32(&acc_empty[b]), (PAIR ? 2 : 1) * kEpiWarps);
     mbar_init(smem_u32(drain), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 0) plan_groups(p, w_tiles, row_first, tile_first, lane);
+  if (warp == 0) plan_groups(p, row_first, tile_first, lane);
   if (warp == 1) {
     if (PAIR) {
       tmem_alloc_pair(smem_u32(tmem_slot), (uint32_t)p.tmem_cols);
@@ -214,59 +287,62 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
   const uint32_t tmem = PAIR ? ld_cluster_u32(mapa_u32(smem_u32(tmem_slot), 0)) : own_tmem;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // Deal units where that is sooner done than whole tiles, the joining of shared tiles included.
-  const int64_t n_tiles_all = tile_first[p.experts], n_units = n_tiles_all * p.k_slabs;
-  const int64_t whole = (n_tiles_all + p.workers - 1) / p.workers * p.k_slabs;
-  const int64_t runs = min((int64_t)p.workers, max(n_units / kMinUnits, (int64_t)1));
-  const bool share = (n_units + runs - 1) / runs + kSplitCost < whole;
-  const int active = (int)(share ? runs : min((int64_t)p.workers, max(n_tiles_all, (int64_t)1)));
-  Schedule sched{row_first, tile_first, 0, 0, Deal(share ? n_units : n_tiles_all, active), p.k_slabs, share};
-  if (worker < active) {
-    const int64_t grain = share ? 1 : p.k_slabs;
-    sched.unit0 = sched.deal.start(worker) * grain, sched.unit1 = sched.deal.start(worker + 1) * grain;
+  // What is left after the full waves is dealt in units where that is sooner done than whole tiles, the
+  // joining of shared tiles included; in so many runs as make the two together least.
+  const int64_t n_all = tile_first[p.experts];
+  int64_t waves = n_all / p.workers;
+  const int left_tiles = (int)(n_all - waves * p.workers);
+  const int64_t left = (int64_t)left_tiles * p.k_slabs;
+  int runs = 0;
+  float least = (float)p.k_slabs;
+  for (int pieces = 1; pieces <= kMaxPieces && left_tiles > 0; pieces++) {
+    const int n = min(p.workers, left_tiles * pieces);
+    const float each = ceilf((float)left / n);
+    const float cost = each + p.join_fixed + p.join_each * (ceilf(p.k_slabs / each) - 1.f);
+    if (each < p.k_slabs && each >= kMinUnits && cost < least) least = cost, runs = n;
   }
+  const int64_t shared0 = waves * p.workers;
+  Schedule sched{row_first, tile_first, worker, (int)waves, shared0, Deal(left, max(runs, 1)), 0, 0};
+  if (runs == 0) sched.waves += shared0 + worker < n_all;       // whole tiles: one more for the first workers
+  else if (worker < runs) sched.u = sched.deal.start(worker), sched.end = sched.deal.start(worker + 1);
   const uint32_t ring = smem_u32(tiles);
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      int s = 0, e = 0;
+      int s = 0;
       uint32_t par = 0;
       int64_t issued = 0;
       bool ok = true;
       // The weights of the first ring are on their way before the codes exist (the launch that makes them
       // lets this one start when all that came before it is done, so weights and group lists are final).
-      const int64_t ahead = min(sched.unit1, sched.unit0 + p.stages);
       for (int pass = 0; pass < 2; pass++) {
-        if (pass) asm volatile("griddepcontrol.wait;" ::: "memory");
-        s = 0, e = 0, par = 0, issued = 0;
-        const int64_t stop = pass ? sched.unit1 : ahead;
-        for (int64_t u = sched.unit0; u < stop && ok;) {
-          const int64_t t = u / p.k_slabs;
-          const Tile tile = tile_at(p, sched, t, e);
-          const int64_t end = min(stop, (t + 1) * p.k_slabs);
+        if (pass) asm volatile("griddepcontrol.wait;" ::: "memory");    // the codes are the previous launch's
+        s = 0, par = 0, issued = 0;
+        Walk walk(sched);
+        Segment g;
+        while (ok && (pass || issued < p.stages) && walk.next(p, sched, g)) {
           // a pair's second half of an odd last weight tile repeats the first; its results are not stored
-          const int nt = PAIR ? min(2 * tile.nt + (int)rank, p.n_tiles - 1) : tile.nt;
-          const int half = PAIR ? ((tile.rows + 31) / 32 * 32) / 2 : 0;
-          const int64_t block0 = ((int64_t)tile.expert * p.n_tiles + nt) * p.k_slabs;
-          for (; u < end; u++) {
+          const int nt = PAIR ? min(2 * g.nt + (int)rank, p.n_tiles - 1) : g.nt;
+          const int half = PAIR ? ((g.rows + 31) / 32 * 32) / 2 : 0;
+          const int64_t block0 = ((int64_t)g.expert * p.n_tiles + nt) * p.k_slabs;
+          for (int ks = g.ks0; ks < g.ks1 && (pass || issued < p.stages); ks++) {
             if (issued >= p.stages && !(ok = mbar_wait(smem_u32(&empty[s]), par ^ 1u, abort_flag, p.status))) break;
-            const int ks = (int)(u - t * p.k_slabs);
             const uint32_t dst = ring + (uint32_t)(s * p.stage_bytes);
             // pair: both CTAs' bytes are counted on the leader's barrier
             const uint32_t bar = PAIR ? mapa_u32(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
-            if (!pass || u >= ahead) {
+            if (!pass || issued >= p.stages) {
               if (PAIR) {
-                mbar_expect_tx_cluster(bar, (uint32_t)p.stage_bytes);
-                tma_load_2d_pair(dst, &tmap_w, 0, (int)((block0 + ks) * 128), bar);
+                mbar_expect_tx_cluster_relaxed(bar, (uint32_t)p.stage_bytes);
+                tma_load_2d_pair(dst, &tmap_w, 0, (int)((block0 + ks) * (kWTile / 1024)), bar);
               } else {
                 mbar_expect_tx(bar, (uint32_t)p.stage_bytes);
                 bulk_load_plain(dst, p.w + (size_t)(block0 + ks) * kWTile, kWTile, bar);
               }
             }
             if (pass) {   // boxes beyond the last row are filled with zeros and count their bytes all the same
-              if (PAIR) tma_load_2d_pair(dst + kWTile, &tmap_a, ks * 128, tile.row0 + (int)rank * half, bar);
-              else tma_load_2d(dst + kWTile, &tmap_a, ks * 128, tile.row0, bar);
+              if (PAIR) tma_load_2d_pair(dst + kWTile, &tmap_a, ks * 128, g.row0 + (int)rank * half, bar);
+              else tma_load_2d(dst + kWTile, &tmap_a, ks * 128, g.row0, bar);
             }
             issued++;
             if (++s == p.stages) s = 0, par ^= 1u;
@@ -284,20 +360,20 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
     if (lane == 0 && rank == 0) {
       const uint64_t desc0 = smem_desc_sw128(ring);
       const uint32_t lo0 = (uint32_t)desc0, hi = (uint32_t)(desc0 >> 32);
-      int s = 0, e = 0, seq = 0;
+      int s = 0, seq = 0;
       uint32_t par = 0;
       bool ok = true;
-      for (int64_t u = sched.unit0; u < sched.unit1 && ok; seq++) {
-        const int64_t t = u / p.k_slabs;
-        const Tile tile = tile_at(p, sched, t, e);
-        const int64_t end = min(sched.unit1, (t + 1) * p.k_slabs);
+      Walk walk(sched);
+      Segment g;
+      for (; ok && walk.next(p, sched, g); seq++) {
         const int b = seq & 1;
-        const int cols = PAIR ? (tile.rows + 31) / 32 * 32 : (tile.rows + 15) / 16 * 16;
+        const int cols = PAIR ? (g.rows + 31) / 32 * 32 : (g.rows + 15) / 16 * 16;
         const uint32_t idesc = p.idesc | (uint32_t)(cols >> 3) << 17;
         const uint32_t acc = tmem + (uint32_t)(b * p.BT);
         if (seq >= 2 && !(ok = mbar_wait(smem_u32(&acc_empty[b]), (uint32_t)((seq >> 1) & 1) ^ 1u, abort_flag, p.status))) break;
         tc_fence_after();
-        for (uint32_t first = 0; u < end; u++, first = 1) {
+        uint32_t first = 0;
+        for (int ks = g.ks0; ks < g.ks1; ks++, first = 1) {
           if (!(ok = mbar_wait(smem_u32(&full[s]), par, abort_flag, p.status))) break;
           tc_fence_after();
           const uint32_t a_lo = lo0 + (uint32_t)((s * p.stage_bytes) >> 4);
@@ -330,77 +406,74 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
     asm volatile("griddepcontrol.wait;" ::: "memory");     // a_max and the counters are the previous launch's
     const int q = warp & 3;                                // TMEM lane quarter this warp may read
     const int ch = q * 32 + lane;                          // channel within the tile
-    int e = 0, seq = 0;
-    for (int64_t u = sched.unit0; u < sched.unit1; seq++) {
-      const int64_t t = u / p.k_slabs;
-      const Tile tile = tile_at(p, sched, t, e);
-      const int64_t tile_u0 = t * p.k_slabs, tile_u1 = tile_u0 + p.k_slabs;
-      const int64_t end = min(sched.unit1, tile_u1);
+    const int c0 = warp >= 2 + 4 ? 32 : 0;                 // first of this warp's chunks, 64 tokens apart
+    int seq = 0;
+    Walk walk(sched);
+    Segment tile;
+    for (; walk.next(p, sched, tile); seq++) {
       const int b = seq & 1;
+      const int nt = PAIR ? 2 * tile.nt + (int)rank : tile.nt;
+      const int n = nt * 128 + ch;
+      const bool alone = tile.ks1 - tile.ks0 == p.k_slabs;
+      const bool mine = nt < p.n_tiles && n < p.N;
+      // what the results need is fetched while the tile is still being multiplied
+      float w_max = nt < p.n_tiles ? p.w_max[((size_t)tile.expert * p.n_tiles + nt) * 128 + ch] : 0.f;
+      float a_max = 0.f;
+      int to = -1;
+      fetch_token(p, tile, c0 + lane, a_max, to);
+      int w0 = 0, others = 0;
+      int* counter = nullptr;
+      if (!alone) {
+        w0 = sched.deal.owner(tile.unit), others = sched.deal.owner(tile.unit + p.k_slabs - 1) - w0;
+        counter = &p.counters[kEpiWarps * (PAIR ? 2 * w0 + (int)rank : w0) + warp - 2];
+      }
       if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[b]), (uint32_t)((seq >> 1) & 1), abort_flag, p.status))) break;
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * p.BT);
-      const int nt = PAIR ? 2 * tile.nt + (int)rank : tile.nt;
-      const bool alone = u == tile_u0 && end == tile_u1;
       bool store = true;
-      int w0 = 0, w1 = 0;
       if (!alone) {
-        // leave the partial sums in this worker's slot; the last of the tile's workers joins them
-        w0 = sched.deal.owner(tile_u0), w1 = sched.deal.owner(tile_u1 - 1);
-        const int cta = PAIR ? 2 * worker + (int)rank : worker;
-        int* slot = p.partial + ((size_t)cta * 2 + (u == tile_u0 ? 1 : 0)) * p.BT * 128 + ch;
-        for (int c = 0; c < tile.rows; c += 32) {
-          uint32_t r[32];
-          tmem_ld32(acc + (uint32_t)c, r);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; i++)
-            if (c + i < tile.rows) slot[(c + i) * 128] = (int)r[i];
-        }
-        // each warp joins its own 32 channels, so no barrier across warps is needed
-        __threadfence();
-        __syncwarp();
+        // Leave the partial sums in this worker's slot; the last of the tile's workers joins them.  Each warp
+        // joins its own channels and chunks, so no barrier across warps is needed.  A worker that finds all
+        // others done is the last and need not write its own sums.
         int seen = 0;
-        if (lane == 0) seen = atomicAdd(&p.counters[4 * (PAIR ? 2 * w0 + (int)rank : w0) + q], 1);
-        store = __shfl_sync(0xffffffffu, seen, 0) == w1 - w0;
+        if (lane == 0) asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+        if (__shfl_sync(0xffffffffu, seen, 0) != others) {
+          const int cta = PAIR ? 2 * worker + (int)rank : worker;
+          int4* slot = p.partial + ((size_t)cta * 2 + (tile.ks0 == 0 ? 1 : 0)) * (p.BT * 32) + ch;
+          for (int c = c0; c < tile.rows; c += 64) {
+            uint32_t r[32];
+            tmem_ld32(acc + (uint32_t)c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int i = 0; i < 32; i += 4)
+              if (c + i < tile.rows)
+                slot[((c + i) >> 2) * 128] = make_int4((int)r[i], (int)r[i + 1], (int)r[i + 2], (int)r[i + 3]);
+          }
+          __threadfence();
+          __syncwarp();
+          if (lane == 0) seen = atomicAdd(counter, 1);
+          store = __shfl_sync(0xffffffffu, seen, 0) == others;
+        }
         __threadfence();
       }
-      const int n = nt * 128 + ch;
       if (store && nt < p.n_tiles) {
-        float w_max = p.w_max[((size_t)tile.expert * p.n_tiles + nt) * 128 + ch];
         const float sw = scale_of(w_max);
         if (sw != sw) w_max = sw;
-        for (int c = 0; c < tile.rows; c += 32) {
+#pragma unroll 1
+        for (int c = c0; c < tile.rows; c += 64) {
           uint32_t r[32];
           tmem_ld32(acc + (uint32_t)c, r);
-          float a_max = 0.f;
-          int to = -1;
-          if (c + lane < tile.rows) {
-            const int row = tile.row0 + c + lane;
-            a_max = p.a_max[row];
-            to = p.order ? p.order[row] : row;
-            if (to >= p.rows) to = -1;
-          }
-          const float sa = scale_of(a_max);
+          const float sa = scale_of(a_max), a_most = a_max;
           const bool plain = __all_sync(0xffffffffu, plain_scale(sa) && plain_scale(sw));
           __syncwarp();
           chunk_sa[lane] = sa, chunk_to[lane] = to;
           __syncwarp();
+          fetch_token(p, tile, c + 64 + lane, a_max, to);        // for the next chunk
           tmem_ld_wait();
-          if (!alone) {
-            for (int w = w0; w <= w1; w++) {
-              if (w == worker) continue;
-              const int cta = PAIR ? 2 * w + (int)rank : w;
-              const int* slot = p.partial + ((size_t)cta * 2 + (w == w0 ? 1 : 0)) * p.BT * 128 + ch;
-#pragma unroll
-              for (int i = 0; i < 32; i++)
-                if (c + i < tile.rows) r[i] += (uint32_t)__ldcg(&slot[(c + i) * 128]);
-            }
-          }
-          const bool mine = n < p.N;
+          if (!alone) join(p, tile, r, c, PAIR ? 2 : 1, (int)rank, worker, w0, others, ch);
+          const int count = tile.rows - c;
+          const int64_t first = tile.row0 + c;
           if (plain) {
-            const int count = tile.rows - c;
-            const int64_t first = tile.row0 + c;
             if (p.out_f16) {
               __half* column = static_cast<__half*>(p.C) + n;
               if (p.order) store_chunk<__half, false>(r, count, chunk_sa, chunk_to, sw, column, 0, p.ldc, mine);
@@ -411,15 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
               else store_chunk<float, true>(r, count, chunk_sa, chunk_to, sw, column, first, p.ldc, mine);
             }
           } else {
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-              const int at = chunk_to[i];
-              const float v = scaled((int)r[i], chunk_sa[i], sw, __shfl_sync(0xffffffffu, a_max, i), w_max);
-              if (at >= 0 && mine) {
-                if (p.out_f16) put(static_cast<__half*>(p.C) + at * p.ldc + n, v);
-                else put(static_cast<float*>(p.C) + at * p.ldc + n, v);
-              }
-            }
+            store_odd(p, r, chunk_sa, chunk_to, sw, a_most, w_max, n, mine);
           }
         }
       }
@@ -429,7 +494,6 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
         if (PAIR) mbar_arrive_cluster(mapa_u32(smem_u32(&acc_empty[b]), 0));
         else mbar_arrive(smem_u32(&acc_empty[b]));
       }
-      u = end;
     }
   }
   // ---------------------------------------------------------------- teardown
@@ -444,20 +508,33 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
 }
 
 // ---------------------------------------------------------------- host side
-// rows of `pitch` bytes (the packed weights: whole blocks, 128-byte rows, already swizzled)
-bool encode_codes(CUtensorMap* map, const void* base, int64_t pitch, int64_t rows, int box_rows, bool swizzle) {
+bool encode_map(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t inner, int64_t rows, int64_t pitch, int box_inner,
+                int box_rows, CUtensorMapSwizzle swizzle) {
   EncodeTiledFn enc = encode_fn();
   if (!enc) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)pitch, (cuuint64_t)rows};
+  const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)pitch};
-  const cuuint32_t box[2] = {128, (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
-  return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+  return enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// token codes [rows][kp], boxes of 128 k in the 128-byte swizzle
+bool encode_codes(CUtensorMap* map, const void* base, int64_t kp, int64_t rows, int box_rows) {
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, base, kp, rows, kp, 128, box_rows, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+// packed weights as lines of 1 KB, sixteen to a block, copied as they are
+constexpr int kBlockLines = kWTile / 1024;
+bool encode_blocks(CUtensorMap* map, const void* base, int64_t blocks) {
+  return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_INT32, base, 256, blocks * kBlockLines, 1024, 256, kBlockLines, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
+
+// What joining a shared tile costs, in units of its main loop: the writing, the counter and the stores once,
+// and the reading of each other worker's sums.
+double join_fixed(bool pair, int bt) { return pair ? 11.0 : 4.0 + 3.0 * bt / 128; }
+double join_each(bool pair, int bt) { return pair ? 7.0 : 0.5 + 2.0 * bt / 128; }
 
 struct Plan {
   bool pair;
@@ -465,18 +542,39 @@ struct Plan {
   size_t codes, maxima, counters, partial;   // bytes of each part of the scratch
 };
 
-// Tokens per tile: a power of two that holds most groups whole (groups differ in size, so twice the mean),
-// and from more than 128 on the pair form, 256 channels by 256 tokens.
-bool make_plan(int64_t rows, int64_t K, int64_t experts, bool groups, Plan* pl) {
+// Tokens per tile.  Few tokens: a power of two that holds most groups whole (groups differ in size, so twice
+// the mean).  More than 128: the pair form, 256 channels by up to 256 tokens; for one matrix the width that
+// leaves the least idle in the last wave, a unit taking 2 clocks per token or the arrival of its bytes
+// at about 88 per clock (24 TB/s over 148 SMs from L2, measured), whichever is longer.
+bool make_plan(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups, Plan* pl) {
   const int64_t mean = (rows + experts - 1) / experts, want = groups ? 2 * mean : mean;
+  pl->ctas = device_sm_count();
   pl->pair = mean > 128;
   pl->bt = 16;
   while (pl->bt < want && pl->bt < 128) pl->bt <<= 1;
-  if (pl->pair) pl->bt = 256;
-  pl->ctas = device_sm_count() & (pl->pair ? ~1 : ~0);
+  if (pl->pair) {
+    pl->ctas &= ~1;
+    pl->bt = 256;
+    double least = 0;
+    const int64_t slabs = (K + 127) / 128, w_tiles = (N + 255) / 256, workers = pl->ctas / 2;
+    for (int64_t tt = (rows + 255) / 256; !groups && tt <= (rows + 127) / 128; tt++) {
+      const int bt = (int)(((rows + tt - 1) / tt + 31) / 32 * 32);
+      const double unit = bt * 2 > (kWTile + bt * 64) / 88 ? bt * 2 : (kWTile + bt * 64) / 88;
+      const int64_t tiles = w_tiles * tt, left = tiles % workers;
+      const double fixed = join_fixed(true, bt), each = join_each(true, bt);
+      double tail = left ? slabs : 0;
+      for (int pieces = 2; left && pieces <= kMaxPieces; pieces++) {
+        const double n = left * pieces < workers ? left * pieces : workers, share = ceil(left * slabs / n);
+        const double cost = share + fixed + each * (ceil(slabs / share) - 1);
+        if (share >= kMinUnits && cost < tail) tail = cost;
+      }
+      const double cost = ((double)(tiles / workers * slabs) + tail) * (unit + 16);
+      if (least == 0 || cost < least) least = cost, pl->bt = bt;
+    }
+  }
   pl->codes = align_up((size_t)rows * align_up((size_t)K, 128), 1024);
   pl->maxima = align_up((size_t)rows * 4, 1024);
-  pl->counters = align_up((size_t)pl->ctas * 16, 1024);
+  pl->counters = align_up((size_t)pl->ctas * kEpiWarps * 4, 1024);
   pl->partial = (size_t)pl->ctas * 2 * pl->bt * 128 * 4;
   return pl->ctas >= 2;
 }
@@ -497,15 +595,15 @@ cudaError_t launch_pdl(void (*kernel)(Args...), int cluster, int ctas, size_t sm
 
 }  // namespace
 
-size_t int8_gemm_workspace_bytes(int64_t rows, int64_t K, int64_t experts, bool groups) {
+size_t int8_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups) {
   Plan pl;
-  if (!make_plan(rows, K, experts, groups, &pl)) return 0;
+  if (!make_plan(rows, N, K, experts, groups, &pl)) return 0;
   return pl.codes + pl.maxima + pl.counters + pl.partial;
 }
 
 cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s) {
   Plan pl;
-  if (!make_plan(g.rows, g.K, g.experts, g.offsets != nullptr, &pl)) return cudaErrorInvalidDevice;
+  if (!make_plan(g.rows, g.N, g.K, g.experts, g.offsets != nullptr, &pl)) return cudaErrorInvalidDevice;
   if (!ws.ptr || ws.bytes < pl.codes + pl.maxima + pl.counters + pl.partial) return cudaErrorInvalidValue;
   const int8_layout l = int8_weight_layout(g.K, g.N, g.experts);
   const int64_t kp = l.k_slabs * 128;
@@ -513,27 +611,30 @@ cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s) {
   float* a_max = reinterpret_cast<float*>(codes + pl.codes);
   int* counters = reinterpret_cast<int*>(codes + pl.codes + pl.maxima);
   cudaError_t e = launch_int8_rows(g.dtype, g.A, g.position ? g.rows / g.fan : g.rows, g.lda, g.K, g.position, g.fan, g.rows,
-                                   codes, a_max, counters, 4 * pl.ctas, s);
+                                   codes, a_max, counters, kEpiWarps * pl.ctas, s);
   if (e != cudaSuccess) return e;
 
   CUtensorMap map_a{}, map_w{};
   const int64_t blocks = l.experts * l.n_tiles * l.k_slabs;
-  if (!encode_codes(&map_a, codes, kp, g.rows, pl.pair ? pl.bt / 2 : pl.bt, true)) return cudaErrorInvalidValue;
-  if (pl.pair && (blocks * 128 > 0x7FFFFFFF || !encode_codes(&map_w, g.W, 128, blocks * 128, 128, false))) return cudaErrorInvalidValue;
+  if (!encode_codes(&map_a, codes, kp, g.rows, pl.pair ? pl.bt / 2 : pl.bt)) return cudaErrorInvalidValue;
+  if (pl.pair && (blocks * kBlockLines > 0x7FFFFFFF || !encode_blocks(&map_w, g.W, blocks))) return cudaErrorInvalidValue;
   Params p{};
   p.w = static_cast<const uint8_t*>(g.W);
   p.w_max = reinterpret_cast<const float*>(p.w + l.code_bytes);
   p.a_max = a_max, p.counters = counters;
-  p.partial = reinterpret_cast<int*>(codes + pl.codes + pl.maxima + pl.counters);
+  p.join_fixed = (float)join_fixed(pl.pair, pl.bt), p.join_each = (float)join_each(pl.pair, pl.bt);
+  p.partial = reinterpret_cast<int4*>(codes + pl.codes + pl.maxima + pl.counters);
   p.offsets = g.offsets, p.order = g.order, p.C = g.C, p.ldc = g.ldc;
   p.rows = (int)g.rows, p.N = (int)g.N, p.experts = (int)g.experts;
   p.n_tiles = (int)l.n_tiles, p.k_slabs = (int)l.k_slabs, p.BT = pl.bt;
+  p.w_tiles = pl.pair ? (p.n_tiles + 1) / 2 : p.n_tiles;
   p.workers = pl.pair ? pl.ctas / 2 : pl.ctas;
   p.header = (int)align_up(kHeader + (size_t)(g.experts + 1) * 8, 1024);
   p.stage_bytes = kWTile + (pl.pair ? pl.bt / 2 : pl.bt) * 128;
   p.stages = (227 * 1024 - p.header) / p.stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
-  p.tmem_cols = 2 * pl.bt < 64 ? 64 : 2 * pl.bt;           // reads go in chunks of 32 columns
+  p.tmem_cols = 64;                                        // a power of two; reads go in chunks of 32 columns
+  while (p.tmem_cols < 2 * pl.bt) p.tmem_cols <<= 1;
   p.out_f16 = g.dtype == kDenseF16;
   // tcgen05.mma kind::i8 instruction descriptor: [4,6) D = s32 (2); [7,10) A and [10,13) B signed 8-bit (1);
   // both operands K-major; [17,23) N >> 3 (per tile); [24,29) M >> 4

@@ -34,11 +34,13 @@ constexpr float kSmallMax = 1e-30f;       // below this 127 / max would leave f3
 // 127 / max, or 0 where no f32 value serves (the f64 lane takes over; `max` must not be 0)
 __device__ __forceinline__ float code_factor(float most) { return most >= kSmallMax ? 127.f / most : 0.f; }
 
+// out of line: reached for one value in 25000, and it would crowd the instruction cache
+__device__ __noinline__ int code_f64(float x, float most) { return (int)rint(__dmul_rn((double)x, 127.0) / (double)most); }
+
 __device__ __forceinline__ int code_of(float x, float most, float factor) {
   const float q = x * factor;
   const float r = rintf(q);
-  if (fabsf(q - r) > kTieMargin || factor == 0.f)
-    return (int)rint(__dmul_rn((double)x, 127.0) / (double)most);
+  if (fabsf(q - r) > kTieMargin || factor == 0.f) return code_f64(x, most);
   return (int)r;
 }
 
@@ -96,45 +98,115 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const T* __restrict__ w,
 }
 
 // ------------------------------------------------------------------------------------ activations, per product
+// kVec consecutive values of a row as f32: one 16-byte load, or (rows that do not start on 16 bytes, the
+// row's end) value by value, zeros beyond K.
+template <typename T>
+struct RowVec;
+template <>
+struct RowVec<float> {
+  static constexpr int kVec = 4;
+  __device__ static void load16(const float* x, float (&v)[4]) {
+    const float4 t = *reinterpret_cast<const float4*>(x);
+    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
+  }
+};
+template <>
+struct RowVec<__half> {
+  static constexpr int kVec = 8;
+  __device__ static void load16(const __half* x, float (&v)[8]) {
+    const uint4 t = *reinterpret_cast<const uint4*>(x);
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+  }
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load_row(const T* x, int64_t k, int64_t K, float (&v)[RowVec<T>::kVec]) {
+  constexpr int kVec = RowVec<T>::kVec;
+  if (WIDE && k + kVec <= K) {
+    RowVec<T>::load16(x + k, v);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kVec; j++) v[j] = k + j < K ? to_f32(x[k + j]) : 0.f;
+  }
+}
+
+// Codes of kVec values as bytes.  One test for all of them decides whether any is near a border.
+template <int kVec>
+__device__ __forceinline__ void make_codes(const float (&v)[kVec], float most, float factor, uint32_t (&word)[kVec / 4]) {
+  int c[kVec];
+  float off = 0.f;
+#pragma unroll
+  for (int j = 0; j < kVec; j++) {
+    const float q = v[j] * factor, r = rintf(q);
+    off = fmaxf(off, fabsf(q - r));
+    c[j] = (int)r;
+  }
+  if (off > kTieMargin || factor == 0.f) {
+#pragma unroll
+    for (int j = 0; j < kVec; j++) c[j] = code_f64(v[j], most);
+  }
+#pragma unroll
+  for (int i = 0; i < kVec / 4; i++)
+    word[i] = (uint32_t)(c[4 * i] & 0xFF) | (uint32_t)(c[4 * i + 1] & 0xFF) << 8 | (uint32_t)(c[4 * i + 2] & 0xFF) << 16 |
+              (uint32_t)(c[4 * i + 3] & 0xFF) << 24;
+}
+
 // One block per row of a: its maximum, then its codes (row-major, rows of kp bytes, zeros from K on) at
 // the row's place, or -- with `position` -- at the `fan` places of the row in a list sorted by expert.
-// A place outside [0, places) is skipped.
-template <typename T>
-__global__ void __launch_bounds__(256) int8_rows_kernel(const T* __restrict__ a, int64_t lda, int64_t K, int64_t kp,
-                                                        const int* __restrict__ position, int fan, int64_t places,
-                                                        uint8_t* __restrict__ codes, float* __restrict__ maxima, int* __restrict__ counters,
-                                                        int n_counters) {
+// A place outside [0, places) is skipped.  The second reading of the row finds it in L1 or L2.
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(1024) int8_rows_kernel(const T* a, int64_t lda, int64_t K, int64_t kp, const int* position, int fan,
+                                                         int64_t places, uint8_t* codes, float* maxima, int* counters,
+                                                         int n_counters) {
+  constexpr int kVec = RowVec<T>::kVec;
   // Wait first, then let the product start: what precedes this launch is finished by then, so the
   // product may read weights and group boundaries before its own wait.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (blockIdx.x == 0)                       // the product's counters of shared tiles start at 0 in every call
-    for (int i = threadIdx.x; i < n_counters; i += 256) counters[i] = 0;
-  __shared__ unsigned warp_most[8];
+    for (int i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
+  __shared__ unsigned warp_most[32];
   const int64_t row = blockIdx.x;
   const T* x = a + row * lda;
+  const int64_t step = (int64_t)blockDim.x * kVec;
   unsigned m = 0;
-  for (int64_t k = threadIdx.x; k < K; k += 256) m = max(m, magnitude(to_f32(x[k])));
+#pragma unroll 4
+  for (int64_t k = (int64_t)threadIdx.x * kVec; k < K; k += step) {
+    float v[kVec];
+    load_row<T, WIDE>(x, k, K, v);
+#pragma unroll
+    for (int j = 0; j < kVec; j++) m = max(m, magnitude(v[j]));
+  }
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; i++) m = max(m, warp_most[i]);
+  m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < (blockDim.x >> 5) ? warp_most[threadIdx.x & 31] : 0u);
   const bool plain = m != 0u && m < kInfBits;
   const float most = __uint_as_float(m), factor = plain ? code_factor(most) : 0.f;
   const int copies = position ? fan : 1;
-  for (int c = threadIdx.x; c < copies; c += 256) {
+  for (int c = threadIdx.x; c < copies; c += blockDim.x) {
     const int64_t at = position ? (int64_t)position[row * fan + c] : row;
     if (at >= 0 && at < places) maxima[at] = __uint_as_float(m < kInfBits ? m : kNaNBits);
   }
-  for (int64_t k = 4 * (int64_t)threadIdx.x; k < kp; k += 1024) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (plain && k + j < K) word |= (uint32_t)(code_of(to_f32(x[k + j]), most, factor) & 0xFF) << (8 * j);
+#pragma unroll 2
+  for (int64_t k = (int64_t)threadIdx.x * kVec; k < kp; k += step) {
+    uint32_t word[kVec / 4] = {};
+    if (plain) {
+      float v[kVec];
+      load_row<T, WIDE>(x, k, K, v);
+      make_codes<kVec>(v, most, factor, word);
+    }
     for (int c = 0; c < copies; c++) {
       const int64_t at = position ? (int64_t)position[row * fan + c] : row;
-      if (at >= 0 && at < places) *reinterpret_cast<uint32_t*>(codes + at * kp + k) = word;
+      if (at < 0 || at >= places) continue;
+      uint32_t* to = reinterpret_cast<uint32_t*>(codes + at * kp + k);
+      if (kVec == 8) *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[kVec / 4 - 1]);
+      else *to = word[0];
     }
   }
 }
@@ -177,18 +249,24 @@ cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda
                              int64_t places, uint8_t* codes, float* maxima, int* counters, int n_counters,
                              cudaStream_t s) {
   const int64_t kp = (K + 127) / 128 * 128;
+  const int es = dtype == kDenseF16 ? 2 : 4;
+  const bool wide = ((reinterpret_cast<uintptr_t>(a) | (uintptr_t)(lda * es)) & 15) == 0;
+  // threads: four 16-byte loads each, two where there are fewer rows than SMs and latency counts
+  const int64_t vecs = (kp * es + 15) / 16, each = rows < device_sm_count() ? 2 : 4;
+  int threads = 64;
+  while (threads < 1024 && threads * each < vecs) threads *= 2;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)rows), cfg.blockDim = dim3(256), cfg.stream = s;
+  cfg.gridDim = dim3((unsigned)rows), cfg.blockDim = dim3((unsigned)threads), cfg.stream = s;
   cfg.attrs = &attr, cfg.numAttrs = 1;
   count_launch();
   if (dtype == kDenseF16)
-    return cudaLaunchKernelEx(&cfg, int8_rows_kernel<__half>, (const __half*)a, lda, K, kp, position, fan, places, codes, maxima,
-                              counters, n_counters);
-  return cudaLaunchKernelEx(&cfg, int8_rows_kernel<float>, (const float*)a, lda, K, kp, position, fan, places, codes, maxima, counters,
-                            n_counters);
+    return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<__half, true> : int8_rows_kernel<__half, false>, (const __half*)a, lda, K,
+                              kp, position, fan, places, codes, maxima, counters, n_counters);
+  return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<float, true> : int8_rows_kernel<float, false>, (const float*)a, lda, K, kp,
+                            position, fan, places, codes, maxima, counters, n_counters);
 }
 
 }  // namespace smith

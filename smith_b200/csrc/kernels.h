@@ -167,7 +167,7 @@ struct Int8Gemm {
   int fan = 1;
   const int* order = nullptr;    // null, or [rows]: sorted row j is row order[j] of C
 };
-size_t int8_gemm_workspace_bytes(int64_t rows, int64_t K, int64_t experts, bool groups);
+size_t int8_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups);
 cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s);
 
 // group_rows.cu : stable counting sort of rows by expert id.

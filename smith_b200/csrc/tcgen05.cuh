@@ -158,6 +158,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cbar) {
 __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t cbar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cbar), "r"(bytes) : "memory");
 }
+// The same without release semantics, for a thread that publishes nothing but the byte count: a release at
+// cluster scope makes the thread wait for its earlier operations, about 0.6 us per arrival.
+__device__ __forceinline__ void mbar_expect_tx_cluster_relaxed(uint32_t cbar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cbar), "r"(bytes) : "memory");
+}
 // tensor-map load into this CTA's shared memory whose bytes are counted on a barrier that may live in the peer CTA
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t cbar) {
   asm volatile(

@@ -43,7 +43,7 @@ constexpr int kWTile = 16384;         // 128 channels x 128 k
 constexpr int kMaxStages = 12;
 constexpr int kHeader = 2560;         // barriers; the group lists follow
 constexpr int kMinUnits = 2;          // fewest units per worker
-constexpr int kMaxPieces = 16;        // most pieces per tile
+constexpr int kMaxPieces = 32;        // most pieces per tile, one lane each
 constexpr int kBlock = 8;             // token tiles side by side
 
 struct Params {
@@ -125,13 +125,14 @@ __device__ __noinline__ void store_odd(const Params& p, const uint32_t (&r)[32],
 
 // ---------------------------------------------------------------- the schedule
 // Equal contiguous runs of `total` units over `workers`: the first total % workers runs hold one more.
+// (At most workers - 1 tiles are dealt, so units count below 2^18.)
 struct Deal {
-  int64_t q, r;
-  __device__ Deal(int64_t total, int workers) : q(total / workers), r(total % workers) {}
-  __device__ int64_t start(int64_t w) const { return w * q + min(w, r); }
-  __device__ int owner(int64_t u) const {
-    const int64_t head = r * (q + 1);
-    return (int)(u < head ? u / (q + 1) : r + (u - head) / q);
+  int q, r;
+  __device__ Deal(int total, int workers) : q(total / workers), r(total - total / workers * workers) {}
+  __device__ int start(int w) const { return w * q + min(w, r); }
+  __device__ int owner(int u) const {
+    const int head = r * (q + 1);
+    return u < head ? u / (q + 1) : r + (u - head) / q;
   }
 };
 
@@ -140,32 +141,32 @@ struct Schedule {
   const int* row_first;     // [experts + 1] cleaned group boundaries
   const int* tile_first;    // [experts + 1] first tile of each group
   int worker, waves;
-  int64_t shared0;          // first tile that may be shared
+  int shared0;              // first tile that may be shared
   Deal deal;                // units from there on
-  int64_t u, end;           // this worker's run of them
+  int u, end;               // this worker's run of them
 };
 
 struct Segment {            // slabs [ks0, ks1) of a tile
   int expert, nt, row0, rows;
   int ks0, ks1;
-  int64_t unit;             // of the tile's slab 0, counted from shared0
+  int unit;                 // of the tile's slab 0, counted from shared0
 };
 
 struct Walk {
   int wave = 0, e = 0;      // tiles only rise, so the group cursor only moves forward
-  int64_t u;
+  int u;
   __device__ explicit Walk(const Schedule& s) : u(s.u) {}
   __device__ __forceinline__ bool next(const Params& p, const Schedule& s, Segment& g) {
-    int64_t t;
+    int t;
     if (wave < s.waves) {
-      t = (int64_t)wave * p.workers + s.worker;
+      t = wave * p.workers + s.worker;
       wave++;
       g.ks0 = 0, g.ks1 = p.k_slabs, g.unit = 0;
     } else {
       if (u >= s.end) return false;
       t = u / p.k_slabs;
       g.unit = t * p.k_slabs;
-      g.ks0 = (int)(u - g.unit), g.ks1 = (int)min((int64_t)p.k_slabs, s.end - g.unit);
+      g.ks0 = u - g.unit, g.ks1 = min(p.k_slabs, s.end - g.unit);
       u = g.unit + g.ks1;
       t += s.shared0;
     }
@@ -174,7 +175,7 @@ struct Walk {
     const int w_tiles = p.w_tiles;
     // blocks of up to kBlock token tiles by all weight tiles, tokens fastest: what runs at one time is
     // compact, so the codes of both sides are fetched by many workers at once
-    const int tt = (count + p.BT - 1) / p.BT, x = (int)t - s.tile_first[e];
+    const int tt = (count + p.BT - 1) / p.BT, x = t - s.tile_first[e];
     const int block = x / (kBlock * w_tiles), in_block = x - block * (kBlock * w_tiles);
     const int width = min(kBlock, tt - block * kBlock);
     g.nt = in_block / width;
@@ -252,6 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
   uint64_t* drain = acc_empty + 2;                         // [1] MMAs in flight, after a give-up
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* plan = reinterpret_cast<int*>(tmem_slot + 2);       // full waves of whole tiles; runs that share the rest (0: none)
   float* chunk_sa = reinterpret_cast<float*>(smem + 512) + ((threadIdx.x >> 5) & 7) * 32;   // [8][32] per epilogue warp
   int* chunk_to = reinterpret_cast<int*>(smem + 512 + 1024) + ((threadIdx.x >> 5) & 7) * 32;
   int* row_first = reinterpret_cast<int*>(smem + kHeader);
@@ -268,7 +270,23 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 0) plan_groups(p, row_first, tile_first, lane);
+  if (warp == 0) {
+    plan_groups(p, row_first, tile_first, lane);
+    __syncwarp();
+    // What is left after the full waves is dealt in units where that is sooner done than whole tiles, the
+    // joining of shared tiles included: lane l looks at l + 1 pieces per tile.
+    const int n_all = tile_first[p.experts], waves = n_all / p.workers, left = n_all - waves * p.workers;
+    const int n = min(p.workers, left * (lane + 1));
+    float cost = (float)p.k_slabs;
+    if (n > 0) {
+      const int each = (left * p.k_slabs + n - 1) / n;
+      if (each >= kMinUnits && each < p.k_slabs)
+        cost = fminf(cost, (float)each + p.join_fixed + p.join_each * (float)((p.k_slabs - 1) / each));
+    }
+    const unsigned bits = __float_as_uint(cost), least = __reduce_min_sync(0xffffffffu, bits);
+    const int best = __ffs(__ballot_sync(0xffffffffu, bits == least)) - 1;
+    if (lane == best) plan[0] = waves, plan[1] = cost < (float)p.k_slabs ? n : 0;
+  }
   if (warp == 1) {
     if (PAIR) {
       tmem_alloc_pair(smem_u32(tmem_slot), (uint32_t)p.tmem_cols);
@@ -287,22 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
   const uint32_t tmem = PAIR ? ld_cluster_u32(mapa_u32(smem_u32(tmem_slot), 0)) : own_tmem;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // What is left after the full waves is dealt in units where that is sooner done than whole tiles, the
-  // joining of shared tiles included; in so many runs as make the two together least.
-  const int64_t n_all = tile_first[p.experts];
-  int64_t waves = n_all / p.workers;
-  const int left_tiles = (int)(n_all - waves * p.workers);
-  const int64_t left = (int64_t)left_tiles * p.k_slabs;
-  int runs = 0;
-  float least = (float)p.k_slabs;
-  for (int pieces = 1; pieces <= kMaxPieces && left_tiles > 0; pieces++) {
-    const int n = min(p.workers, left_tiles * pieces);
-    const float each = ceilf((float)left / n);
-    const float cost = each + p.join_fixed + p.join_each * (ceilf(p.k_slabs / each) - 1.f);
-    if (each < p.k_slabs && each >= kMinUnits && cost < least) least = cost, runs = n;
-  }
-  const int64_t shared0 = waves * p.workers;
-  Schedule sched{row_first, tile_first, worker, (int)waves, shared0, Deal(left, max(runs, 1)), 0, 0};
+  const int waves = plan[0], runs = plan[1], n_all = tile_first[p.experts], shared0 = waves * p.workers;
+  Schedule sched{row_first, tile_first, worker, waves, shared0, Deal((n_all - shared0) * p.k_slabs, max(runs, 1)), 0, 0};
   if (runs == 0) sched.waves += shared0 + worker < n_all;       // whole tiles: one more for the first workers
   else if (worker < runs) sched.u = sched.deal.start(worker), sched.end = sched.deal.start(worker + 1);
   const uint32_t ring = smem_u32(tiles);
@@ -544,8 +548,10 @@ struct Plan {
 
 // Tokens per tile.  Few tokens: a power of two that holds most groups whole (groups differ in size, so twice
 // the mean).  More than 128: the pair form, 256 channels by up to 256 tokens; for one matrix the width that
-// leaves the least idle in the last wave, a unit taking 2 clocks per token or the arrival of its bytes
-// at about 88 per clock (24 TB/s over 148 SMs from L2, measured), whichever is longer.
+// leaves the least idle in the last wave.  A unit takes 2 clocks per token and a part that does not shrink
+// with the width: at full rate the board is at its power limit, and the weights' way through L2 costs the
+// same for a narrow tile (measured at 4096 x 4096 x 14336: 256 wide 229 us, the narrower tile that an equal
+// price per token would choose 290 us).
 bool make_plan(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups, Plan* pl) {
   const int64_t mean = (rows + experts - 1) / experts, want = groups ? 2 * mean : mean;
   pl->ctas = device_sm_count();
@@ -559,7 +565,6 @@ bool make_plan(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups,
     const int64_t slabs = (K + 127) / 128, w_tiles = (N + 255) / 256, workers = pl->ctas / 2;
     for (int64_t tt = (rows + 255) / 256; !groups && tt <= (rows + 127) / 128; tt++) {
       const int bt = (int)(((rows + tt - 1) / tt + 31) / 32 * 32);
-      const double unit = bt * 2 > (kWTile + bt * 64) / 88 ? bt * 2 : (kWTile + bt * 64) / 88;
       const int64_t tiles = w_tiles * tt, left = tiles % workers;
       const double fixed = join_fixed(true, bt), each = join_each(true, bt);
       double tail = left ? slabs : 0;
@@ -568,7 +573,7 @@ bool make_plan(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups,
         const double cost = share + fixed + each * (ceil(slabs / share) - 1);
         if (share >= kMinUnits && cost < tail) tail = cost;
       }
-      const double cost = ((double)(tiles / workers * slabs) + tail) * (unit + 16);
+      const double cost = ((double)(tiles / workers * slabs) + tail) * (bt * 2 + 130);
       if (least == 0 || cost < least) least = cost, pl->bt = bt;
     }
   }

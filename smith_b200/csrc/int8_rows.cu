@@ -8,12 +8,14 @@
 // kept beside the codes is the maximum (f32, exact; NaN for a vector that is not finite), from which the
 // product forms the scale.
 //
-// A code is evaluated in f32 and checked: q = x * (127 / max) carries two roundings, |q| <= 127, so it is
-// within 127 * (2^-23 + 2^-48) < 1.6e-5 of the real quotient.  Unless q lies closer than 2e-5 to the
-// middle between two codes (one value in 25000) the nearest integer to q is the code; otherwise, and for
-// vectors so small that 127 / max leaves f32, the quotient is formed in f64: 127 * x is exact there, and
-// a quotient of a 31-bit and a 24-bit number that is no half-integer differs from every half-integer by
-// far more than an f64 rounding, so the result is the definition's in every case.
+// A code is evaluated in f32 and checked.  t = fma(x, f, 1.5 * 2^23) with f = f32(127 / max) rounds x * f to
+// a whole number (half to even) in t's low bits; x * f is within 127 * 2^-24 < 8e-6 of the real quotient.
+// Unless x * f lies closer than 2e-5 to the middle between two codes (one value in 25000) that is the
+// code; otherwise the sign of 254 x - (2 low + 1) max, low being the code below, decides: each product is
+// an f32 and its exact remainder (fma), the f32 parts are close and subtract exactly, and the remainders
+// have few enough bits to do so too, so the sign is exact.  Vectors whose maximum is below 2^-90 or above
+// 2^90 are multiplied by 2^100 or 2^-100 first, so that nothing leaves f32's range (what underflows there
+// has code 0 anyway).  Conversions (f32 to integer, rint) would run at an eighth of the rate.
 //
 // Packed weights (built for the tensor cores' operand fetch): expert e, channel tile nt (128 channels),
 // slab ks (128 k) is one contiguous block of 16 KB at ((e * NT + nt) * KS + ks) * 16384; channel r of the
@@ -29,19 +31,37 @@ namespace smith {
 namespace {
 
 constexpr float kTieMargin = 0.49998f;    // 0.5 - 2e-5, see above
-constexpr float kSmallMax = 1e-30f;       // below this 127 / max would leave f32's range soon: all in f64
+constexpr float kMagic = 12582912.f;      // 1.5 * 2^23: adding it leaves the nearest whole number in the low bits
 
-// 127 / max, or 0 where no f32 value serves (the f64 lane takes over; `max` must not be 0)
-__device__ __forceinline__ float code_factor(float most) { return most >= kSmallMax ? 127.f / most : 0.f; }
+// How a vector's codes are made, from its maximum (finite and not 0): x * lift * factor.
+struct Coder {
+  float most, lift, factor;
+  __device__ explicit Coder(float m) : lift(m < 0x1p-90f ? 0x1p100f : m > 0x1p90f ? 0x1p-100f : 1.f) {
+    most = m * lift;
+    factor = 127.f / most;
+  }
+};
 
-// out of line: reached for one value in 25000, and it would crowd the instruction cache
-__device__ __noinline__ int code_f64(float x, float most) { return (int)rint(__dmul_rn((double)x, 127.0) / (double)most); }
+// x (lifted) near the middle of two codes
+__device__ __forceinline__ uint32_t code_near_border(float x, const Coder& c) {
+  const float low = floorf(x * c.factor), odd = 2.f * low + 1.f;
+  const float a = 254.f * x, b = odd * c.most;
+  const float over = (a - b) + (fmaf(254.f, x, -a) - fmaf(odd, c.most, -b));
+  const int l = (int)low;
+  return (uint32_t)(l + (over > 0.f || (over == 0.f && (l & 1)) ? 1 : 0));
+}
 
-__device__ __forceinline__ int code_of(float x, float most, float factor) {
-  const float q = x * factor;
-  const float r = rintf(q);
-  if (fabsf(q - r) > kTieMargin || factor == 0.f) return code_f64(x, most);
-  return (int)r;
+// The code in the low byte; off = distance of x * factor from it.
+__device__ __forceinline__ uint32_t code_bits(float x, float factor, float& off) {
+  const float t = fmaf(x, factor, kMagic);
+  off = fabsf(fmaf(x, factor, kMagic - t));
+  return __float_as_uint(t);
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, const Coder& c) {
+  float off;
+  const uint32_t bits = code_bits(x * c.lift, c.factor, off);
+  return (off > kTieMargin ? code_near_border(x * c.lift, c) : bits) & 0xFFu;
 }
 
 // bits of |x| order like |x| among non-negative f32, infinities above and NaNs above those
@@ -80,14 +100,14 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const T* __restrict__ w,
   const unsigned bits = n < N ? most[e * n_pad + n] : 0u;
   const float m = __uint_as_float(bits);
   const bool plain = bits != 0u && bits < kInfBits;
-  const float factor = plain ? code_factor(m) : 0.f;
+  const Coder coder(plain ? m : 1.f);
   const T* col = w + e * K * N + n;
   for (int q = threadIdx.x >> 7; q < 32; q += 2) {   // four k each
     uint32_t word = 0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       const int64_t k = ks * 128 + 4 * q + j;
-      if (plain && k < K) word |= (uint32_t)(code_of(to_f32(col[k * N]), m, factor) & 0xFF) << (8 * j);
+      if (plain && k < K) word |= code_of(to_f32(col[k * N]), coder) << (8 * j);
     }
     block[r * 32 + (((q >> 2) ^ (r & 7)) << 2) + (q & 3)] = word;
   }
@@ -98,117 +118,145 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const T* __restrict__ w,
 }
 
 // ------------------------------------------------------------------------------------ activations, per product
-// kVec consecutive values of a row as f32: one 16-byte load, or (rows that do not start on 16 bytes, the
-// row's end) value by value, zeros beyond K.
-template <typename T>
-struct RowVec;
-template <>
-struct RowVec<float> {
-  static constexpr int kVec = 4;
-  __device__ static void load16(const float* x, float (&v)[4]) {
-    const float4 t = *reinterpret_cast<const float4*>(x);
-    v[0] = t.x, v[1] = t.y, v[2] = t.z, v[3] = t.w;
-  }
-};
-template <>
-struct RowVec<__half> {
-  static constexpr int kVec = 8;
-  __device__ static void load16(const __half* x, float (&v)[8]) {
-    const uint4 t = *reinterpret_cast<const uint4*>(x);
-    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+// Sixteen bytes of a row from element k: one load, or (rows that do not start on 16 bytes, the row's end)
+// value by value, zeros beyond K.
+template <typename T, bool WIDE>
+__device__ __forceinline__ uint4 load16(const T* x, int k, int K) {
+  constexpr int kVec = 16 / sizeof(T);
+  if (WIDE && k + kVec <= K) return *reinterpret_cast<const uint4*>(x + k);
+  uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  for (int i = 0; i < 4; i++) {
+    if (sizeof(T) == 4) {
+      w[i] = k + i < K ? reinterpret_cast<const uint32_t*>(x)[k + i] : 0u;
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(x) + k + 2 * i;
+      w[i] = (k + 2 * i < K ? (uint32_t)h[0] : 0u) | (k + 2 * i + 1 < K ? (uint32_t)h[1] << 16 : 0u);
     }
   }
-};
-
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load_row(const T* x, int64_t k, int64_t K, float (&v)[RowVec<T>::kVec]) {
-  constexpr int kVec = RowVec<T>::kVec;
-  if (WIDE && k + kVec <= K) {
-    RowVec<T>::load16(x + k, v);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kVec; j++) v[j] = k + j < K ? to_f32(x[k + j]) : 0.f;
-  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Codes of kVec values as bytes.  One test for all of them decides whether any is near a border.
-template <int kVec>
-__device__ __forceinline__ void make_codes(const float (&v)[kVec], float most, float factor, uint32_t (&word)[kVec / 4]) {
-  int c[kVec];
+// Running maximum of magnitudes as bits (halves: two in a word); infinities and NaNs are the largest.
+template <typename T>
+__device__ __forceinline__ void take_most(uint32_t& m, const uint4& v) {
+  for (const uint32_t w : {v.x, v.y, v.z, v.w}) m = sizeof(T) == 4 ? max(m, w & 0x7FFFFFFFu) : __vmaxu2(m, w & 0x7FFF7FFFu);
+}
+
+// {lo, hi} pairs: two f32 operations in one instruction
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Codes of sixteen bytes of values.  One test for all of them decides whether any is near a border.
+template <typename T>
+__device__ __forceinline__ void make_codes(const uint4& raw, const Coder& coder, uint32_t (&word)[4 / sizeof(T)]) {
+  constexpr int kVec = 16 / sizeof(T);
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  float x[kVec];
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (sizeof(T) == 4) {
+      x[i] = __uint_as_float(w[i]);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      x[(2 * i) % kVec] = f.x, x[(2 * i + 1) % kVec] = f.y;
+    }
+  }
+  if (coder.lift != 1.f) {
+#pragma unroll
+    for (int j = 0; j < kVec; j++) x[j] *= coder.lift;
+  }
+  const uint64_t f2 = pair_of(coder.factor, coder.factor), magic2 = pair_of(kMagic, kMagic), minus2 = pair_of(-1.f, -1.f);
+  uint32_t c[kVec];
   float off = 0.f;
 #pragma unroll
-  for (int j = 0; j < kVec; j++) {
-    const float q = v[j] * factor, r = rintf(q);
-    off = fmaxf(off, fabsf(q - r));
-    c[j] = (int)r;
+  for (int j = 0; j < kVec; j += 2) {
+    const uint64_t x2 = pair_of(x[j], x[j + 1]), t2 = fma2(x2, f2, magic2);
+    float t0, t1, d0, d1;
+    unpair(t2, t0, t1);
+    unpair(fma2(x2, f2, fma2(t2, minus2, magic2)), d0, d1);
+    c[j] = __float_as_uint(t0), c[j + 1] = __float_as_uint(t1);
+    off = fmaxf(off, fmaxf(fabsf(d0), fabsf(d1)));
   }
-  if (off > kTieMargin || factor == 0.f) {
+  if (off > kTieMargin) {
 #pragma unroll
-    for (int j = 0; j < kVec; j++) c[j] = code_f64(v[j], most);
+    for (int j = 0; j < kVec; j++) {
+      float d;
+      code_bits(x[j], coder.factor, d);
+      if (d > kTieMargin) c[j] = code_near_border(x[j], coder);
+    }
   }
 #pragma unroll
   for (int i = 0; i < kVec / 4; i++)
-    word[i] = (uint32_t)(c[4 * i] & 0xFF) | (uint32_t)(c[4 * i + 1] & 0xFF) << 8 | (uint32_t)(c[4 * i + 2] & 0xFF) << 16 |
-              (uint32_t)(c[4 * i + 3] & 0xFF) << 24;
+    word[i] = __byte_perm(__byte_perm(c[4 * i], c[4 * i + 1], 0x0040), __byte_perm(c[4 * i + 2], c[4 * i + 3], 0x0040), 0x5410);
 }
 
 // One block per row of a: its maximum, then its codes (row-major, rows of kp bytes, zeros from K on) at
 // the row's place, or -- with `position` -- at the `fan` places of the row in a list sorted by expert.
-// A place outside [0, places) is skipped.  The second reading of the row finds it in L1 or L2.
+// A place outside [0, places) is skipped.  Bound by reading the row and by instructions (about six per
+// value), so each thread keeps its first kHeld vectors in registers; a longer row is read again.
+constexpr int kHeld = 8;
 template <typename T, bool WIDE>
-__global__ void __launch_bounds__(1024) int8_rows_kernel(const T* a, int64_t lda, int64_t K, int64_t kp, const int* position, int fan,
-                                                         int64_t places, uint8_t* codes, float* maxima, int* counters,
-                                                         int n_counters) {
-  constexpr int kVec = RowVec<T>::kVec;
+__global__ void __launch_bounds__(256) int8_rows_kernel(const T* a, int64_t lda, int K, int kp, const int* position, int fan,
+                                                        int places, uint8_t* codes, float* maxima, int* counters, int n_counters) {
+  constexpr int kVec = 16 / sizeof(T);
   // Wait first, then let the product start: what precedes this launch is finished by then, so the
   // product may read weights and group boundaries before its own wait.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (blockIdx.x == 0)                       // the product's counters of shared tiles start at 0 in every call
-    for (int i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
-  __shared__ unsigned warp_most[32];
   const int64_t row = blockIdx.x;
   const T* x = a + row * lda;
-  const int64_t step = (int64_t)blockDim.x * kVec;
-  unsigned m = 0;
-#pragma unroll 4
-  for (int64_t k = (int64_t)threadIdx.x * kVec; k < K; k += step) {
-    float v[kVec];
-    load_row<T, WIDE>(x, k, K, v);
+  const int first = threadIdx.x * kVec, step = blockDim.x * kVec;
+  uint4 held[kHeld];
 #pragma unroll
-    for (int j = 0; j < kVec; j++) m = max(m, magnitude(v[j]));
-  }
+  for (int i = 0; i < kHeld; i++) held[i] = first + i * step < K ? load16<T, WIDE>(x, first + i * step, K) : make_uint4(0, 0, 0, 0);
+  if (blockIdx.x == 0)                       // the product's counters of shared tiles start at 0 in every call
+    for (int i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
+  __shared__ unsigned warp_most[8];
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < kHeld; i++) take_most<T>(m, held[i]);
+#pragma unroll 4
+  for (int k = first + kHeld * step; k < K; k += step) take_most<T>(m, load16<T, WIDE>(x, k, K));
+  if (sizeof(T) == 2) m = max(m & 0xFFFFu, m >> 16);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
   __syncthreads();
-  m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < (blockDim.x >> 5) ? warp_most[threadIdx.x & 31] : 0u);
+#pragma unroll
+  for (int i = 0; i < 8; i++)
+    if (i < (int)(blockDim.x >> 5)) m = max(m, warp_most[i]);
+  if (sizeof(T) == 2) m = m >= 0x7C00u ? kNaNBits : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
   const bool plain = m != 0u && m < kInfBits;
-  const float most = __uint_as_float(m), factor = plain ? code_factor(most) : 0.f;
+  const Coder coder(plain ? __uint_as_float(m) : 1.f);
   const int copies = position ? fan : 1;
   for (int c = threadIdx.x; c < copies; c += blockDim.x) {
-    const int64_t at = position ? (int64_t)position[row * fan + c] : row;
+    const int at = position ? position[row * fan + c] : (int)row;
     if (at >= 0 && at < places) maxima[at] = __uint_as_float(m < kInfBits ? m : kNaNBits);
   }
-#pragma unroll 2
-  for (int64_t k = (int64_t)threadIdx.x * kVec; k < kp; k += step) {
+  auto put_codes = [&](int k, const uint4& raw) {
     uint32_t word[kVec / 4] = {};
-    if (plain) {
-      float v[kVec];
-      load_row<T, WIDE>(x, k, K, v);
-      make_codes<kVec>(v, most, factor, word);
-    }
+    if (plain) make_codes<T>(raw, coder, word);
     for (int c = 0; c < copies; c++) {
-      const int64_t at = position ? (int64_t)position[row * fan + c] : row;
+      const int at = position ? position[row * fan + c] : (int)row;
       if (at < 0 || at >= places) continue;
-      uint32_t* to = reinterpret_cast<uint32_t*>(codes + at * kp + k);
+      uint32_t* to = reinterpret_cast<uint32_t*>(codes + (int64_t)at * kp + k);
       if (kVec == 8) *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[kVec / 4 - 1]);
       else *to = word[0];
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < kHeld; i++)
+    if (first + i * step < kp) put_codes(first + i * step, held[i]);
+  for (int k = first + kHeld * step; k < kp; k += step) put_codes(k, k < K ? load16<T, WIDE>(x, k, K) : make_uint4(0, 0, 0, 0));
 }
 
 }  // namespace
@@ -251,22 +299,35 @@ cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda
   const int64_t kp = (K + 127) / 128 * 128;
   const int es = dtype == kDenseF16 ? 2 : 4;
   const bool wide = ((reinterpret_cast<uintptr_t>(a) | (uintptr_t)(lda * es)) & 15) == 0;
-  // threads: four 16-byte loads each, two where there are fewer rows than SMs and latency counts
-  const int64_t vecs = (kp * es + 15) / 16, each = rows < device_sm_count() ? 2 : 4;
+  // threads: four 16-byte loads each; at most 256, so that a block of the product fits beside on its SM
+  const int64_t vecs = (kp * es + 15) / 16;
   int threads = 64;
-  while (threads < 1024 && threads * each < vecs) threads *= 2;
+  while (threads < 256 && threads * 4 < vecs) threads *= 2;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
+  // The product takes nearly all of an SM's shared memory.  These blocks ask for the same split of L1 and
+  // shared memory, else an SM would have to drain before it could take a block of the product.
+  static PerDeviceFlag configured;
+  bool* set = configured.here();
+  if (!set) return cudaErrorInvalidDevice;
+  if (!*set) {
+    for (const void* k : {(const void*)int8_rows_kernel<__half, true>, (const void*)int8_rows_kernel<__half, false>,
+                          (const void*)int8_rows_kernel<float, true>, (const void*)int8_rows_kernel<float, false>}) {
+      const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+      if (e != cudaSuccess) return e;
+    }
+    *set = true;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows), cfg.blockDim = dim3((unsigned)threads), cfg.stream = s;
   cfg.attrs = &attr, cfg.numAttrs = 1;
   count_launch();
   if (dtype == kDenseF16)
-    return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<__half, true> : int8_rows_kernel<__half, false>, (const __half*)a, lda, K,
-                              kp, position, fan, places, codes, maxima, counters, n_counters);
-  return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<float, true> : int8_rows_kernel<float, false>, (const float*)a, lda, K, kp,
-                            position, fan, places, codes, maxima, counters, n_counters);
+    return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<__half, true> : int8_rows_kernel<__half, false>, (const __half*)a, lda, (int)K,
+                              (int)kp, position, fan, (int)places, codes, maxima, counters, n_counters);
+  return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<float, true> : int8_rows_kernel<float, false>, (const float*)a, lda, (int)K, (int)kp,
+                            position, fan, (int)places, codes, maxima, counters, n_counters);
 }
 
 }  // namespace smith

@@ -306,7 +306,8 @@ int do_group_rows(Context* c, const int* ids, int* offsets, int* order, int* pos
       if (overlap(out[i], bytes[i], out[j], bytes[j])) return fail("group_rows: outputs overlap");
   }
   if (reinterpret_cast<uintptr_t>(ids) & 3) return fail("group_rows: buffers must be aligned to 4 bytes");
-  cudaError_t e = launch_group_rows(ids, (int64_t)rows, (int64_t)experts, offsets, order, position, c->stream);
+  if (ensure_int8_workspace(c, group_rows_workspace_bytes((int64_t)rows, (int64_t)experts))) return 1;
+  cudaError_t e = launch_group_rows(ids, (int64_t)rows, (int64_t)experts, offsets, order, position, c->int8_ws, c->stream);
   return e == cudaSuccess ? 0 : fail("group_rows launch failed: %s", cudaGetErrorString(e));
 }
 

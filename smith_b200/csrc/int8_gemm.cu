@@ -186,17 +186,14 @@ struct Walk {
 };
 
 // Group boundaries come from device memory: clamped and made to rise, so that nothing they hold leads
-// outside the rows or covers a row twice.  One warp; tiles of a group = weight tiles x token tiles.
+// outside the rows or covers a row twice.  One warp, on row_first as all threads fetched it; tiles of a
+// group = weight tiles x token tiles.
 __device__ __forceinline__ void plan_groups(const Params& p, int* row_first, int* tile_first, int lane) {
   int high = 0, tiles = 0;
   if (lane == 0) tile_first[0] = 0;
-  if (!p.offsets) {
-    if (lane == 0) row_first[0] = 0, row_first[1] = p.rows, tile_first[1] = p.w_tiles * ((p.rows + p.BT - 1) / p.BT);
-    return;
-  }
   for (int i0 = 0; i0 <= p.experts; i0 += 32) {
     const int i = i0 + lane;
-    int v = i <= p.experts ? min(max(p.offsets[i], 0), p.rows) : 0;
+    int v = i <= p.experts ? row_first[i] : 0;
     for (int d = 1; d < 32; d <<= 1) v = max(v, (int)__shfl_up_sync(0xffffffffu, v, d) * (lane >= d ? 1 : 0));
     v = max(v, high);
     int before = __shfl_up_sync(0xffffffffu, v, 1);
@@ -242,7 +239,7 @@ __device__ __forceinline__ void join(const Params& p, const Segment& tile, uint3
 }
 
 template <bool PAIR>
-__global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
+__global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
                                                                 const __grid_constant__ CUtensorMap tmap_w,
                                                                 const __grid_constant__ Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -270,6 +267,18 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  for (int i = tid; i <= p.experts; i += kThreads)
+    row_first[i] = p.offsets ? min(max(p.offsets[i], 0), p.rows) : (i ? p.rows : 0);
+  if (warp == 1) {
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), (uint32_t)p.tmem_cols);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), (uint32_t)p.tmem_cols);
+      tmem_relinquish();
+    }
+  }
+  __syncthreads();
   if (warp == 0) {
     plan_groups(p, row_first, tile_first, lane);
     __syncwarp();
@@ -286,15 +295,6 @@ __global__ void __launch_bounds__(kThreads, 1) int8_gemm_kernel(const __grid_con
     const unsigned bits = __float_as_uint(cost), least = __reduce_min_sync(0xffffffffu, bits);
     const int best = __ffs(__ballot_sync(0xffffffffu, bits == least)) - 1;
     if (lane == best) plan[0] = waves, plan[1] = cost < (float)p.k_slabs ? n : 0;
-  }
-  if (warp == 1) {
-    if (PAIR) {
-      tmem_alloc_pair(smem_u32(tmem_slot), (uint32_t)p.tmem_cols);
-      tmem_relinquish_pair();
-    } else {
-      tmem_alloc(smem_u32(tmem_slot), (uint32_t)p.tmem_cols);
-      tmem_relinquish();
-    }
   }
   tc_fence_before();
   __syncthreads();

@@ -202,11 +202,18 @@ __device__ __forceinline__ void make_codes(const uint4& raw, const Coder& coder,
 
 // One block per row of a: its maximum, then its codes (row-major, rows of kp bytes, zeros from K on) at
 // the row's place, or -- with `position` -- at the `fan` places of the row in a list sorted by expert.
-// A place outside [0, places) is skipped.  Bound by reading the row and by instructions (about six per
-// value), so each thread keeps its first kHeld vectors in registers; a longer row is read again.
-constexpr int kHeld = 8;
-template <typename T, bool WIDE>
-__global__ void __launch_bounds__(256) int8_rows_kernel(const T* a, int64_t lda, int K, int kp, const int* position, int fan,
+// A place outside [0, places) is skipped.  Each thread keeps its first HELD vectors in registers; what a
+// longer row has beyond is read again.
+//
+// Two forms.  Many rows are bound by reading them and by instructions (about six per value): 256 threads
+// and 8 vectors in flight each.  Rows fewer than SMs are bound by latency: 512 threads with 2 vectors each
+// are through soonest (one row of 4096 f32: 128 threads 5.6 us until the product could begin, 256 threads
+// 3.1 us), and with at most 32 registers a thread, so that a block of the product finds room beside (a
+// quarter of an SM's register file holds three of its ten warps; with more registers here, the SMs that
+// hold one of these blocks began the product 2.5 to 5 us late).
+constexpr int kNearPlaces = 32;
+template <typename T, bool WIDE, int HELD, int THREADS>
+__global__ void __launch_bounds__(THREADS, HELD == 2 ? 4 : 1) int8_rows_kernel(const T* a, int64_t lda, int K, int kp, const int* position, int fan,
                                                         int places, uint8_t* codes, float* maxima, int* counters, int n_counters) {
   constexpr int kVec = 16 / sizeof(T);
   // Wait first, then let the product start: what precedes this launch is finished by then, so the
@@ -216,37 +223,37 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const T* a, int64_t lda,
   const int64_t row = blockIdx.x;
   const T* x = a + row * lda;
   const int first = threadIdx.x * kVec, step = blockDim.x * kVec;
-  uint4 held[kHeld];
+  uint4 held[HELD];
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) held[i] = first + i * step < K ? load16<T, WIDE>(x, first + i * step, K) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < HELD; i++) held[i] = first + i * step < K ? load16<T, WIDE>(x, first + i * step, K) : make_uint4(0, 0, 0, 0);
   if (blockIdx.x == 0)                       // the product's counters of shared tiles start at 0 in every call
     for (int i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
-  __shared__ unsigned warp_most[8];
+  __shared__ unsigned warp_most[THREADS / 32];
+  __shared__ int near_places[kNearPlaces];   // the row's places, fetched while its values are on their way
+  if (threadIdx.x < kNearPlaces) near_places[threadIdx.x] = !position ? (int)row : threadIdx.x < fan ? position[row * fan + threadIdx.x] : -1;
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < kHeld; i++) take_most<T>(m, held[i]);
+  for (int i = 0; i < HELD; i++) take_most<T>(m, held[i]);
 #pragma unroll 4
-  for (int k = first + kHeld * step; k < K; k += step) take_most<T>(m, load16<T, WIDE>(x, k, K));
+  for (int k = first + HELD * step; k < K; k += step) take_most<T>(m, load16<T, WIDE>(x, k, K));
   if (sizeof(T) == 2) m = max(m & 0xFFFFu, m >> 16);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; i++)
-    if (i < (int)(blockDim.x >> 5)) m = max(m, warp_most[i]);
+  m = __reduce_max_sync(0xffffffffu, (threadIdx.x & 31) < (blockDim.x >> 5) ? warp_most[threadIdx.x & 31] : 0u);
   if (sizeof(T) == 2) m = m >= 0x7C00u ? kNaNBits : __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
   const bool plain = m != 0u && m < kInfBits;
   const Coder coder(plain ? __uint_as_float(m) : 1.f);
   const int copies = position ? fan : 1;
   for (int c = threadIdx.x; c < copies; c += blockDim.x) {
-    const int at = position ? position[row * fan + c] : (int)row;
+    const int at = c < kNearPlaces ? near_places[c] : position[row * fan + c];
     if (at >= 0 && at < places) maxima[at] = __uint_as_float(m < kInfBits ? m : kNaNBits);
   }
   auto put_codes = [&](int k, const uint4& raw) {
     uint32_t word[kVec / 4] = {};
     if (plain) make_codes<T>(raw, coder, word);
     for (int c = 0; c < copies; c++) {
-      const int at = position ? position[row * fan + c] : (int)row;
+      const int at = c < kNearPlaces ? near_places[c] : position[row * fan + c];
       if (at < 0 || at >= places) continue;
       uint32_t* to = reinterpret_cast<uint32_t*>(codes + (int64_t)at * kp + k);
       if (kVec == 8) *reinterpret_cast<uint2*>(to) = make_uint2(word[0], word[kVec / 4 - 1]);
@@ -254,9 +261,9 @@ __global__ void __launch_bounds__(256) int8_rows_kernel(const T* a, int64_t lda,
     }
   };
 #pragma unroll
-  for (int i = 0; i < kHeld; i++)
+  for (int i = 0; i < HELD; i++)
     if (first + i * step < kp) put_codes(first + i * step, held[i]);
-  for (int k = first + kHeld * step; k < kp; k += step) put_codes(k, k < K ? load16<T, WIDE>(x, k, K) : make_uint4(0, 0, 0, 0));
+  for (int k = first + HELD * step; k < kp; k += step) put_codes(k, k < K ? load16<T, WIDE>(x, k, K) : make_uint4(0, 0, 0, 0));
 }
 
 }  // namespace
@@ -299,35 +306,38 @@ cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda
   const int64_t kp = (K + 127) / 128 * 128;
   const int es = dtype == kDenseF16 ? 2 : 4;
   const bool wide = ((reinterpret_cast<uintptr_t>(a) | (uintptr_t)(lda * es)) & 15) == 0;
-  // threads: four 16-byte loads each; at most 256, so that a block of the product fits beside on its SM
+  const bool few = rows < device_sm_count();
   const int64_t vecs = (kp * es + 15) / 16;
   int threads = 64;
-  while (threads < 256 && threads * 4 < vecs) threads *= 2;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+  while (threads < (few ? 512 : 256) && threads * (few ? 2 : 4) < vecs) threads *= 2;
+  using Kernel = void (*)(const void*, int64_t, int, int, const int*, int, int, uint8_t*, float*, int*, int);
+  static const Kernel kernels[8] = {
+      (Kernel)int8_rows_kernel<float, false, 8, 256>,  (Kernel)int8_rows_kernel<float, false, 2, 512>,
+      (Kernel)int8_rows_kernel<float, true, 8, 256>,   (Kernel)int8_rows_kernel<float, true, 2, 512>,
+      (Kernel)int8_rows_kernel<__half, false, 8, 256>, (Kernel)int8_rows_kernel<__half, false, 2, 512>,
+      (Kernel)int8_rows_kernel<__half, true, 8, 256>,  (Kernel)int8_rows_kernel<__half, true, 2, 512>};
   // The product takes nearly all of an SM's shared memory.  These blocks ask for the same split of L1 and
-  // shared memory, else an SM would have to drain before it could take a block of the product.
+  // shared memory, else an SM might have to drain before it could take a block of the product.
   static PerDeviceFlag configured;
   bool* set = configured.here();
   if (!set) return cudaErrorInvalidDevice;
   if (!*set) {
-    for (const void* k : {(const void*)int8_rows_kernel<__half, true>, (const void*)int8_rows_kernel<__half, false>,
-                          (const void*)int8_rows_kernel<float, true>, (const void*)int8_rows_kernel<float, false>}) {
-      const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    for (Kernel k : kernels) {
+      const cudaError_t e = cudaFuncSetAttribute((const void*)k, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
       if (e != cudaSuccess) return e;
     }
     *set = true;
   }
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)rows), cfg.blockDim = dim3((unsigned)threads), cfg.stream = s;
   cfg.attrs = &attr, cfg.numAttrs = 1;
   count_launch();
-  if (dtype == kDenseF16)
-    return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<__half, true> : int8_rows_kernel<__half, false>, (const __half*)a, lda, (int)K,
-                              (int)kp, position, fan, (int)places, codes, maxima, counters, n_counters);
-  return cudaLaunchKernelEx(&cfg, wide ? int8_rows_kernel<float, true> : int8_rows_kernel<float, false>, (const float*)a, lda, (int)K, (int)kp,
-                            position, fan, (int)places, codes, maxima, counters, n_counters);
+  int ikp = (int)kp, iK = (int)K, iplaces = (int)places;
+  void* args[] = {&a, &lda, &iK, &ikp, &position, &fan, &iplaces, &codes, &maxima, &counters, &n_counters};
+  return cudaLaunchKernelExC(&cfg, (const void*)kernels[(dtype == kDenseF16 ? 4 : 0) + (wide ? 2 : 0) + (few ? 1 : 0)], args);
 }
 
 }  // namespace smith

@@ -171,8 +171,9 @@ size_t int8_gemm_workspace_bytes(int64_t rows, int64_t N, int64_t K, int64_t exp
 cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s);
 
 // group_rows.cu : stable counting sort of rows by expert id.
+size_t group_rows_workspace_bytes(int64_t rows, int64_t experts);
 cudaError_t launch_group_rows(const int* ids, int64_t rows, int64_t experts, int* offsets, int* order, int* position,
-                              cudaStream_t s);
+                              Workspace ws, cudaStream_t s);
 
 // util.cu
 // Number of SMs of the current device (cached per device; 148 if the query fails).

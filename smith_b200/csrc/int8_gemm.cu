@@ -21,7 +21,7 @@
 //
 //   warp 0     producer: one copy of the packed 16 KB weight block and one box of token codes per unit
 //   warp 1     MMA issuer; two accumulators in tensor memory, so the next tile runs during an epilogue
-//   warps 2-9  epilogue: two warps share a quarter of the lanes and take its 32-token chunks in turn
+//   warps 2-9  epilogue: two warps share a quarter of the lanes, each takes half of the tile's tokens
 // Every mbarrier wait is time-bounded (pipeline.cuh); on a give-up the CTA waits (bounded) for its copies
 // and MMAs in flight, frees its tensor memory and leaves the status word set.
 #include <cuda.h>
@@ -41,9 +41,9 @@ constexpr int kEpiWarps = 8;
 constexpr int kThreads = (2 + kEpiWarps) * 32;
 constexpr int kWTile = 16384;         // 128 channels x 128 k
 constexpr int kMaxStages = 12;
-constexpr int kHeader = 2560;         // barriers; the group lists follow
+constexpr int kWarpTokens = 128;      // most tokens of one epilogue warp: half of a tile
+constexpr int kHeader = 512 + kEpiWarps * kWarpTokens * 8;        // barriers; the group lists follow
 constexpr int kMinUnits = 2;          // fewest units per worker
-constexpr int kMaxPieces = 32;        // most pieces per tile, one lane each
 constexpr int kBlock = 8;             // token tiles side by side
 
 struct Params {
@@ -55,7 +55,7 @@ struct Params {
   void* C;
   int4* partial;                      // two slots of [BT / 4][128] per CTA
   int* counters;                      // one per epilogue warp of each CTA
-  float join_fixed, join_each;        // what joining a shared tile costs, in units: once, and per worker joined
+  float alone, join_fixed, join_each; // see Costs
   int64_t ldc;
   int rows, N, experts;
   int n_tiles, k_slabs;
@@ -84,14 +84,15 @@ __device__ __noinline__ float scaled(int sum, float sa, float sw, float a_max, f
 __device__ __forceinline__ void put(float* at, float v) { __stcs(at, v); }
 __device__ __forceinline__ void put(__half* at, float v) { __stcs(at, __float2half_rn(v)); }
 
-// Up to 32 tokens of one channel: sums r scaled and stored; sa and to (row of C, negative: none) are the
-// chunk's in shared memory.  `first` is the chunk's first row of C where rows are in order.
+// Eight tokens of one channel: sums r scaled and stored; sa and to (row of C, negative: none) are the
+// tokens' in shared memory.  `at` is the first token's place in C where rows are in order.  (Eight at a
+// time in a loop: code that runs once or twice per launch is paid for by its length.  Unrolled to 32 tokens
+// the epilogue of a small product took 3 us.)
 template <typename T, bool ORDERED>
-__device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], int count, const float* sa, const int* to, float sw, T* column,
-                                            int64_t first, int64_t ldc, bool mine) {
-  T* at = column + first * ldc;
+__device__ __forceinline__ void store_tokens(const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw, T* column,
+                                             T* at, int64_t ldc, bool mine) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 4) {
+  for (int i = 0; i < 8; i += 4) {
     const float4 s4 = *reinterpret_cast<const float4*>(sa + i);
     const float s[4] = {s4.x, s4.y, s4.z, s4.w};
     int4 t4 = make_int4(0, 0, 0, 0);
@@ -103,23 +104,23 @@ __device__ __forceinline__ void store_chunk(const uint32_t (&r)[32], int count, 
       if (ORDERED) {
         if (mine && i + j < count) put(at, v);
         at += ldc;
-      } else if (mine && t[j] >= 0) {
+      } else if (mine && i + j < count && t[j] >= 0) {
         put(column + t[j] * ldc, v);
       }
     }
   }
 }
 
-// The same for a chunk with a scale outside the plain range; rare, so kept out of line.
-__device__ __noinline__ void store_odd(const Params& p, const uint32_t (&r)[32], const float* sa, const int* to, float sw, float a_max,
-                                       float w_max, int n, bool mine) {
+// The same where a scale is outside the plain range; rare, so kept out of line.
+__device__ __noinline__ void store_odd(const Params& p, const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw,
+                                       float w_max, int row, int n, bool mine) {
 #pragma unroll
-  for (int i = 0; i < 32; i++) {
-    const float v = scaled((int)r[i], sa[i], sw, __shfl_sync(0xffffffffu, a_max, i), w_max);
-    if (to[i] >= 0 && mine) {
-      if (p.out_f16) put(static_cast<__half*>(p.C) + to[i] * p.ldc + n, v);
-      else put(static_cast<float*>(p.C) + to[i] * p.ldc + n, v);
-    }
+  for (int i = 0; i < 8; i++) {
+    if (i >= count || to[i] < 0 || !mine) continue;
+    const float a_max = p.a_max[row + i];
+    const float v = scaled((int)r[i], sa[i], sw, a_max, w_max);
+    if (p.out_f16) put(static_cast<__half*>(p.C) + to[i] * p.ldc + n, v);
+    else put(static_cast<float*>(p.C) + to[i] * p.ldc + n, v);
   }
 }
 
@@ -142,6 +143,7 @@ struct Schedule {
   const int* tile_first;    // [experts + 1] first tile of each group
   int worker, waves;
   int shared0;              // first tile that may be shared
+  int pieces;               // workers per shared tile; 0: runs go over tile borders
   Deal deal;                // units from there on
   int u, end;               // this worker's run of them
 };
@@ -186,7 +188,7 @@ struct Walk {
 };
 
 // Group boundaries come from device memory: clamped and made to rise, so that nothing they hold leads
-// outside the rows or covers a row twice.  One warp, on row_first as all threads fetched it; tiles of a
+// outside the rows or covers a row twice.  One warp, on row_first as fetched; tiles of a
 // group = weight tiles x token tiles.
 __device__ __forceinline__ void plan_groups(const Params& p, int* row_first, int* tile_first, int lane) {
   int high = 0, tiles = 0;
@@ -210,30 +212,16 @@ __device__ __forceinline__ void plan_groups(const Params& p, int* row_first, int
   }
 }
 
-// Token c of a tile: its maximum and its row of C (-1: none).
-__device__ __forceinline__ void fetch_token(const Params& p, const Segment& tile, int c, float& a_max, int& to) {
-  a_max = 0.f, to = -1;
-  if (c < tile.rows) {
-    const int row = tile.row0 + c;
-    a_max = p.a_max[row];
-    to = p.order ? p.order[row] : row;
-    if (to >= p.rows) to = -1;
-  }
-}
-
-// Adds the partial sums of a tile's other workers to one chunk.
-__device__ __forceinline__ void join(const Params& p, const Segment& tile, uint32_t (&r)[32], int c, int ctas, int rank, int worker, int w0,
-                                     int others, int ch) {
-#pragma unroll 2
+// Adds the partial sums of a tile's other workers to eight tokens.
+__device__ __forceinline__ void join(const Params& p, uint32_t (&r)[8], int c, int ctas, int rank, int worker, int w0, int others, int ch) {
+#pragma unroll 4
   for (int k = 0; k < others; k++) {
     const int w = w0 + k + (w0 + k >= worker ? 1 : 0);
     const int4* slot = p.partial + ((size_t)(ctas * w + rank) * 2 + (w == w0 ? 1 : 0)) * (p.BT * 32) + (c >> 2) * 128 + ch;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      if (c + 4 * i < tile.rows) {
-        const int4 v = __ldcg(&slot[i * 128]);
-        r[4 * i] += (uint32_t)v.x, r[4 * i + 1] += (uint32_t)v.y, r[4 * i + 2] += (uint32_t)v.z, r[4 * i + 3] += (uint32_t)v.w;
-      }
+    for (int i = 0; i < 2; i++) {
+      const int4 v = __ldcg(&slot[i * 128]);
+      r[4 * i] += (uint32_t)v.x, r[4 * i + 1] += (uint32_t)v.y, r[4 * i + 2] += (uint32_t)v.z, r[4 * i + 3] += (uint32_t)v.w;
     }
   }
 }
@@ -250,9 +238,10 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
   uint64_t* drain = acc_empty + 2;                         // [1] MMAs in flight, after a give-up
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* plan = reinterpret_cast<int*>(tmem_slot + 2);       // full waves of whole tiles; runs that share the rest (0: none)
-  float* chunk_sa = reinterpret_cast<float*>(smem + 512) + ((threadIdx.x >> 5) & 7) * 32;   // [8][32] per epilogue warp
-  int* chunk_to = reinterpret_cast<int*>(smem + 512 + 1024) + ((threadIdx.x >> 5) & 7) * 32;
+  int* plan = reinterpret_cast<int*>(tmem_slot + 2);       // full waves of whole tiles; workers per tile of the rest (-1: runs)
+  // per epilogue warp: scale and row of C of each of its tokens
+  float* tok_sa = reinterpret_cast<float*>(smem + 512) + ((threadIdx.x >> 5) & 7) * kWarpTokens;
+  int* tok_to = reinterpret_cast<int*>(smem + 512 + kEpiWarps * kWarpTokens * 4) + ((threadIdx.x >> 5) & 7) * kWarpTokens;
   int* row_first = reinterpret_cast<int*>(smem + kHeader);
   int* tile_first = row_first + p.experts + 1;
   uint8_t* tiles = smem + p.header;
@@ -260,15 +249,13 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;    // 0: the CTA that issues the pair's MMAs
   const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x;
 
-  if (tid == 0) {
+  if (tid == 64) {
     for (int s = 0; s < kMaxStages; s++) mbar_init(smem_u32(&full[s]), PAIR ? 2 : 1), mbar_init(smem_u32(&empty[s]), 1);
     for (int b = 0; b < 2; b++) mbar_init(smem_u32(&acc_full[b]), 1), mbar_init(smem_u32(&acc_empty[b]), (PAIR ? 2 : 1) * kEpiWarps);
     mbar_init(smem_u32(drain), 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  for (int i = tid; i <= p.experts; i += kThreads)
-    row_first[i] = p.offsets ? min(max(p.offsets[i], 0), p.rows) : (i ? p.rows : 0);
   if (warp == 1) {
     if (PAIR) {
       tmem_alloc_pair(smem_u32(tmem_slot), (uint32_t)p.tmem_cols);
@@ -278,23 +265,30 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
       tmem_relinquish();
     }
   }
-  __syncthreads();
   if (warp == 0) {
+#pragma unroll 4
+    for (int i = lane; i <= p.experts; i += 32) row_first[i] = p.offsets ? min(max(p.offsets[i], 0), p.rows) : (i ? p.rows : 0);
+    __syncwarp();
     plan_groups(p, row_first, tile_first, lane);
     __syncwarp();
-    // What is left after the full waves is dealt in units where that is sooner done than whole tiles, the
-    // joining of shared tiles included: lane l looks at l + 1 pieces per tile.
+    // What is left after the full waves: whole tiles (lane 0), l + 1 workers per tile (lane l), or runs of
+    // units over all workers (lane 31), whichever is done first.  A worker alone moves its units faster
+    // than its share of the memory's rate (p.alone), so few workers can be enough; joining costs
+    // p.join_fixed units per shared tile of a worker and p.join_each per other worker of the tile.
     const int n_all = tile_first[p.experts], waves = n_all / p.workers, left = n_all - waves * p.workers;
-    const int n = min(p.workers, left * (lane + 1));
-    float cost = (float)p.k_slabs;
-    if (n > 0) {
-      const int each = (left * p.k_slabs + n - 1) / n;
-      if (each >= kMinUnits && each < p.k_slabs)
-        cost = fminf(cost, (float)each + p.join_fixed + p.join_each * (float)((p.k_slabs - 1) / each));
+    const int all = left * p.k_slabs;
+    int each = (p.k_slabs + lane) / (lane + 1);
+    float joins = lane == 0 ? 0.f : p.join_fixed + p.join_each * (float)lane;
+    bool can = left * (lane + 1) <= p.workers && lane < p.k_slabs;
+    if (lane == 31) {
+      each = (all + p.workers - 1) / p.workers;
+      can = each >= kMinUnits;
+      joins = 2.f * p.join_fixed + p.join_each * (float)(1 + p.k_slabs / max(each, 1));
     }
+    const float cost = can ? fmaxf((float)all / (float)p.workers, p.alone * (float)each) + joins : 1e30f;
     const unsigned bits = __float_as_uint(cost), least = __reduce_min_sync(0xffffffffu, bits);
     const int best = __ffs(__ballot_sync(0xffffffffu, bits == least)) - 1;
-    if (lane == best) plan[0] = waves, plan[1] = cost < (float)p.k_slabs ? n : 0;
+    if (lane == best) plan[0] = waves, plan[1] = lane == 31 ? -1 : lane + 1;
   }
   tc_fence_before();
   __syncthreads();
@@ -305,10 +299,18 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
   const uint32_t tmem = PAIR ? ld_cluster_u32(mapa_u32(smem_u32(tmem_slot), 0)) : own_tmem;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int waves = plan[0], runs = plan[1], n_all = tile_first[p.experts], shared0 = waves * p.workers;
-  Schedule sched{row_first, tile_first, worker, waves, shared0, Deal((n_all - shared0) * p.k_slabs, max(runs, 1)), 0, 0};
-  if (runs == 0) sched.waves += shared0 + worker < n_all;       // whole tiles: one more for the first workers
-  else if (worker < runs) sched.u = sched.deal.start(worker), sched.end = sched.deal.start(worker + 1);
+  const int waves = plan[0], pieces = plan[1], n_all = tile_first[p.experts], shared0 = waves * p.workers;
+  const int left = n_all - shared0;
+  Schedule sched{row_first, tile_first, worker, waves, shared0, max(pieces, 0), Deal(left * p.k_slabs, p.workers), 0, 0};
+  if (pieces < 0) {                                             // runs over all units
+    sched.u = sched.deal.start(worker), sched.end = sched.deal.start(worker + 1);
+  } else if (pieces > 1) {
+    const int t = worker / pieces;
+    const Deal slabs(p.k_slabs, pieces);
+    if (t < left) sched.u = t * p.k_slabs + slabs.start(worker - t * pieces), sched.end = t * p.k_slabs + slabs.start(worker - t * pieces + 1);
+  } else {
+    sched.waves += shared0 + worker < n_all;                    // whole tiles: one more for the first workers
+  }
   const uint32_t ring = smem_u32(tiles);
 
   if (warp == 0) {
@@ -361,11 +363,11 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (pair: the leader's only)
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {
       const uint64_t desc0 = smem_desc_sw128(ring);
-      const uint32_t lo0 = (uint32_t)desc0, hi = (uint32_t)(desc0 >> 32);
+      const uint32_t lo0 = (uint32_t)desc0, hi = (uint32_t)(desc0 >> 32), step = (uint32_t)p.stage_bytes >> 4;
       int s = 0, seq = 0;
-      uint32_t par = 0;
+      uint32_t par = 0, a_lo = lo0;
       bool ok = true;
       Walk walk(sched);
       Segment g;
@@ -374,34 +376,31 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
         const int cols = PAIR ? (g.rows + 31) / 32 * 32 : (g.rows + 15) / 16 * 16;
         const uint32_t idesc = p.idesc | (uint32_t)(cols >> 3) << 17;
         const uint32_t acc = tmem + (uint32_t)(b * p.BT);
-        if (seq >= 2 && !(ok = mbar_wait(smem_u32(&acc_empty[b]), (uint32_t)((seq >> 1) & 1) ^ 1u, abort_flag, p.status))) break;
+        if (seq >= 2) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_empty[b]), (uint32_t)((seq >> 1) & 1) ^ 1u, abort_flag, p.status));
+        if (!ok) break;
         tc_fence_after();
         uint32_t first = 0;
         for (int ks = g.ks0; ks < g.ks1; ks++, first = 1) {
-          if (!(ok = mbar_wait(smem_u32(&full[s]), par, abort_flag, p.status))) break;
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), par, abort_flag, p.status));
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a_lo = lo0 + (uint32_t)((s * p.stage_bytes) >> 4);
           if (PAIR) {
             umma_i8_kblock_pair(acc, a_lo, a_lo + (kWTile >> 4), hi, idesc, first);
-            umma_commit_pair(smem_u32(&empty[s]));
-            umma_commit_pair(mapa_u32(smem_u32(&empty[s]), 1));
+            umma_commit_both_elected(smem_u32(&empty[s]));
           } else {
             umma_i8_kblock(acc, a_lo, a_lo + (kWTile >> 4), hi, idesc, first);
-            umma_commit(smem_u32(&empty[s]));
+            umma_commit_elected(smem_u32(&empty[s]));
           }
-          if (++s == p.stages) s = 0, par ^= 1u;
+          a_lo += step;
+          if (++s == p.stages) s = 0, par ^= 1u, a_lo = lo0;
         }
         if (!ok) break;
-        if (PAIR) {
-          umma_commit_pair(smem_u32(&acc_full[b]));
-          umma_commit_pair(mapa_u32(smem_u32(&acc_full[b]), 1));
-        } else {
-          umma_commit(smem_u32(&acc_full[b]));
-        }
+        if (PAIR) umma_commit_both_elected(smem_u32(&acc_full[b]));
+        else umma_commit_elected(smem_u32(&acc_full[b]));
       }
       if (!ok) {
-        if (PAIR) umma_commit_pair(smem_u32(drain));
-        else umma_commit(smem_u32(drain));
+        if (PAIR) umma_commit_both_elected(smem_u32(drain));
+        else umma_commit_elected(smem_u32(drain));
         for (int spin = 0; spin < 100000 && !mbar_try(smem_u32(drain), 0); spin++) {}
       }
     }
@@ -410,7 +409,7 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
     asm volatile("griddepcontrol.wait;" ::: "memory");     // a_max and the counters are the previous launch's
     const int q = warp & 3;                                // TMEM lane quarter this warp may read
     const int ch = q * 32 + lane;                          // channel within the tile
-    const int c0 = warp >= 2 + 4 ? 32 : 0;                 // first of this warp's chunks, 64 tokens apart
+    const bool second = warp >= 2 + 4;                     // of the two warps of this quarter
     int seq = 0;
     Walk walk(sched);
     Segment tile;
@@ -420,76 +419,82 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
       const int n = nt * 128 + ch;
       const bool alone = tile.ks1 - tile.ks0 == p.k_slabs;
       const bool mine = nt < p.n_tiles && n < p.N;
+      const int half = ((tile.rows + 1) / 2 + 7) & ~7;
+      const int c0 = second ? half : 0, c1 = second ? tile.rows : min(half, tile.rows);
       // what the results need is fetched while the tile is still being multiplied
-      float w_max = nt < p.n_tiles ? p.w_max[((size_t)tile.expert * p.n_tiles + nt) * 128 + ch] : 0.f;
-      float a_max = 0.f;
-      int to = -1;
-      fetch_token(p, tile, c0 + lane, a_max, to);
-      int w0 = 0, others = 0;
+      float w_max = mine ? p.w_max[((size_t)tile.expert * p.n_tiles + nt) * 128 + ch] : 0.f;
+      const float sw = scale_of(w_max);
+      if (sw != sw) w_max = sw;
+      bool plain = plain_scale(sw);
+      __syncwarp();
+      for (int i = lane; c0 + i < c1; i += 32) {
+        const int row = tile.row0 + c0 + i;
+        const float sa = scale_of(p.a_max[row]);
+        const int to = p.order ? p.order[row] : row;
+        tok_sa[i] = sa, tok_to[i] = to < p.rows ? to : -1;
+        plain = plain && plain_scale(sa);
+      }
+      plain = __all_sync(0xffffffffu, plain);
+      __syncwarp();
+      int w0 = 0, others = 0, seen = 0;
       int* counter = nullptr;
       if (!alone) {
-        w0 = sched.deal.owner(tile.unit), others = sched.deal.owner(tile.unit + p.k_slabs - 1) - w0;
+        if (sched.pieces) w0 = tile.unit / p.k_slabs * sched.pieces, others = sched.pieces - 1;
+        else w0 = sched.deal.owner(tile.unit), others = sched.deal.owner(tile.unit + p.k_slabs - 1) - w0;
         counter = &p.counters[kEpiWarps * (PAIR ? 2 * w0 + (int)rank : w0) + warp - 2];
+        if (lane == 0) asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
+        seen = __shfl_sync(0xffffffffu, seen, 0);
       }
       if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&acc_full[b]), (uint32_t)((seq >> 1) & 1), abort_flag, p.status))) break;
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(b * p.BT);
-      bool store = true;
-      if (!alone) {
+      bool store = c0 < c1;
+      if (!alone && c0 < c1) {
         // Leave the partial sums in this worker's slot; the last of the tile's workers joins them.  Each warp
-        // joins its own channels and chunks, so no barrier across warps is needed.  A worker that finds all
+        // joins its own channels and tokens, so no barrier across warps is needed.  A worker that finds all
         // others done is the last and need not write its own sums.
-        int seen = 0;
-        if (lane == 0) asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(seen) : "l"(counter) : "memory");
-        if (__shfl_sync(0xffffffffu, seen, 0) != others) {
+        if (seen != others) {
           const int cta = PAIR ? 2 * worker + (int)rank : worker;
           int4* slot = p.partial + ((size_t)cta * 2 + (tile.ks0 == 0 ? 1 : 0)) * (p.BT * 32) + ch;
-          for (int c = c0; c < tile.rows; c += 64) {
-            uint32_t r[32];
-            tmem_ld32(acc + (uint32_t)c, r);
+#pragma unroll 1
+          for (int c = c0; c < c1; c += 8) {
+            uint32_t r[8];
+            tmem_ld8(acc + (uint32_t)c, r);
             tmem_ld_wait();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              if (c + i < tile.rows)
-                slot[((c + i) >> 2) * 128] = make_int4((int)r[i], (int)r[i + 1], (int)r[i + 2], (int)r[i + 3]);
+            for (int i = 0; i < 8; i += 4)
+              slot[((c + i) >> 2) * 128] = make_int4((int)r[i], (int)r[i + 1], (int)r[i + 2], (int)r[i + 3]);
           }
           __threadfence();
           __syncwarp();
           if (lane == 0) seen = atomicAdd(counter, 1);
           store = __shfl_sync(0xffffffffu, seen, 0) == others;
         }
-        __threadfence();
+        if (store) __threadfence();
       }
       if (store && nt < p.n_tiles) {
-        const float sw = scale_of(w_max);
-        if (sw != sw) w_max = sw;
+        int64_t at = (int64_t)(tile.row0 + c0) * p.ldc + n;
 #pragma unroll 1
-        for (int c = c0; c < tile.rows; c += 64) {
-          uint32_t r[32];
-          tmem_ld32(acc + (uint32_t)c, r);
-          const float sa = scale_of(a_max), a_most = a_max;
-          const bool plain = __all_sync(0xffffffffu, plain_scale(sa) && plain_scale(sw));
-          __syncwarp();
-          chunk_sa[lane] = sa, chunk_to[lane] = to;
-          __syncwarp();
-          fetch_token(p, tile, c + 64 + lane, a_max, to);        // for the next chunk
+        for (int c = c0; c < c1; c += 8) {
+          uint32_t r[8];
+          tmem_ld8(acc + (uint32_t)c, r);
           tmem_ld_wait();
-          if (!alone) join(p, tile, r, c, PAIR ? 2 : 1, (int)rank, worker, w0, others, ch);
-          const int count = tile.rows - c;
-          const int64_t first = tile.row0 + c;
-          if (plain) {
-            if (p.out_f16) {
-              __half* column = static_cast<__half*>(p.C) + n;
-              if (p.order) store_chunk<__half, false>(r, count, chunk_sa, chunk_to, sw, column, 0, p.ldc, mine);
-              else store_chunk<__half, true>(r, count, chunk_sa, chunk_to, sw, column, first, p.ldc, mine);
-            } else {
-              float* column = static_cast<float*>(p.C) + n;
-              if (p.order) store_chunk<float, false>(r, count, chunk_sa, chunk_to, sw, column, 0, p.ldc, mine);
-              else store_chunk<float, true>(r, count, chunk_sa, chunk_to, sw, column, first, p.ldc, mine);
-            }
+          if (!alone) join(p, r, c, PAIR ? 2 : 1, (int)rank, worker, w0, others, ch);
+          const float* sa = tok_sa + (c - c0);
+          const int* to = tok_to + (c - c0);
+          const int count = c1 - c;
+          if (!plain) {
+            store_odd(p, r, count, sa, to, sw, w_max, tile.row0 + c, n, mine);
+          } else if (p.out_f16) {
+            __half* C = static_cast<__half*>(p.C);
+            if (p.order) store_tokens<__half, false>(r, count, sa, to, sw, C + n, C, p.ldc, mine);
+            else store_tokens<__half, true>(r, count, sa, to, sw, C, C + at, p.ldc, mine);
           } else {
-            store_odd(p, r, chunk_sa, chunk_to, sw, a_most, w_max, n, mine);
+            float* C = static_cast<float*>(p.C);
+            if (p.order) store_tokens<float, false>(r, count, sa, to, sw, C + n, C, p.ldc, mine);
+            else store_tokens<float, true>(r, count, sa, to, sw, C, C + at, p.ldc, mine);
           }
+          at += 8 * p.ldc;
         }
       }
       tc_fence_before();
@@ -535,10 +540,13 @@ bool encode_blocks(CUtensorMap* map, const void* base, int64_t blocks) {
 
 size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
-// What joining a shared tile costs, in units of its main loop: the writing, the counter and the stores once,
-// and the reading of each other worker's sums.
-double join_fixed(bool pair, int bt) { return pair ? 11.0 : 4.0 + 3.0 * bt / 128; }
-double join_each(bool pair, int bt) { return pair ? 7.0 : 0.5 + 2.0 * bt / 128; }
+// In units of the main loop (0.28 us for a pair at 256 tokens, bound by the tensor cores; 0.37 us for one
+// CTA of 148 that stream weights): the time of a unit when few workers are active, what a worker pays once
+// for a shared tile (writing, the counter, the stores), and for the sums of each other worker.
+struct Costs {
+  double alone, join_fixed, join_each;
+  Costs(bool pair, int bt) : alone(pair ? 1.0 : 0.75), join_fixed(pair ? 11.0 : 4.0 + 3.0 * bt / 128), join_each(pair ? 7.0 : 0.5 + 2.0 * bt / 128) {}
+};
 
 struct Plan {
   bool pair;
@@ -566,13 +574,15 @@ bool make_plan(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups,
     for (int64_t tt = (rows + 255) / 256; !groups && tt <= (rows + 127) / 128; tt++) {
       const int bt = (int)(((rows + tt - 1) / tt + 31) / 32 * 32);
       const int64_t tiles = w_tiles * tt, left = tiles % workers;
-      const double fixed = join_fixed(true, bt), each = join_each(true, bt);
-      double tail = left ? slabs : 0;
-      for (int pieces = 2; left && pieces <= kMaxPieces; pieces++) {
-        const double n = left * pieces < workers ? left * pieces : workers, share = ceil(left * slabs / n);
-        const double cost = share + fixed + each * (ceil(slabs / share) - 1);
-        if (share >= kMinUnits && cost < tail) tail = cost;
+      const Costs c(true, bt);
+      double tail = left ? (double)slabs : 0;
+      for (int64_t pieces = 2; left && left * pieces <= workers && pieces <= slabs; pieces++) {
+        const double t = (double)((slabs + pieces - 1) / pieces) + c.join_fixed + c.join_each * (pieces - 1);
+        if (t < tail) tail = t;
       }
+      const double run = ceil((double)(left * slabs) / workers);
+      if (left && run >= kMinUnits && run + 2 * c.join_fixed + c.join_each * (1 + slabs / run) < tail)
+        tail = run + 2 * c.join_fixed + c.join_each * (1 + slabs / run);
       const double cost = ((double)(tiles / workers * slabs) + tail) * (bt * 2 + 130);
       if (least == 0 || cost < least) least = cost, pl->bt = bt;
     }
@@ -627,7 +637,8 @@ cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s) {
   p.w = static_cast<const uint8_t*>(g.W);
   p.w_max = reinterpret_cast<const float*>(p.w + l.code_bytes);
   p.a_max = a_max, p.counters = counters;
-  p.join_fixed = (float)join_fixed(pl.pair, pl.bt), p.join_each = (float)join_each(pl.pair, pl.bt);
+  const Costs costs(pl.pair, pl.bt);
+  p.alone = (float)costs.alone, p.join_fixed = (float)costs.join_fixed, p.join_each = (float)costs.join_each;
   p.partial = reinterpret_cast<int4*>(codes + pl.codes + pl.maxima + pl.counters);
   p.offsets = g.offsets, p.order = g.order, p.C = g.C, p.ldc = g.ldc;
   p.rows = (int)g.rows, p.N = (int)g.N, p.experts = (int)g.experts;

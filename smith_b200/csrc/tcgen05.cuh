@@ -65,34 +65,38 @@ __device__ __forceinline__ void umma_f16_kblock(uint32_t d_tmem, uint32_t a_lo, 
       "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
       : "memory");
 }
-// The four MMAs of one 128-byte slab of 8-bit integers (D s32): 128 k, 128 x N x 32 each.
+// The four MMAs of one 128-byte slab of 8-bit integers (D s32): 128 k, 128 x N x 32 each.  Called by a whole
+// converged warp, one elected lane issues (always the same, which also commits): with the loop around it
+// uniform over the warp, the descriptors stay in uniform registers.  Issued from a branch of one lane, the
+// four MMAs and their commits took 383 clocks, against 512 of tensor work for a pair's 256 x 256 x 128.
 __device__ __forceinline__ void umma_i8_kblock(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi,
                                                uint32_t idesc, uint32_t accumulate_first) {
   asm volatile(
       "{\n"
-      ".reg .pred p, q;\n"
+      ".reg .pred e, p, q;\n"
       ".reg .b32 ta, tb;\n"
       ".reg .b64 da, db;\n"
+      "elect.sync _|e, 0xffffffff;\n"
       "setp.ne.b32 p, %5, 0;\n"
-      "setp.ne.b32 q, %4, 0;\n"
+      "setp.ne.b32 q, %4, 0;\n"          // the instruction descriptor is never zero: q = true
       "mov.b64 da, {%1, %3};\n"
       "mov.b64 db, {%2, %3};\n"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, p;\n"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, p;\n"
       "add.u32 ta, %1, 2;\n"
       "add.u32 tb, %2, 2;\n"
       "mov.b64 da, {ta, %3};\n"
       "mov.b64 db, {tb, %3};\n"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
       "add.u32 ta, %1, 4;\n"
       "add.u32 tb, %2, 4;\n"
       "mov.b64 da, {ta, %3};\n"
       "mov.b64 db, {tb, %3};\n"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
       "add.u32 ta, %1, 6;\n"
       "add.u32 tb, %2, 6;\n"
       "mov.b64 da, {ta, %3};\n"
       "mov.b64 db, {tb, %3};\n"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
+      "@e tcgen05.mma.cta_group::1.kind::i8 [%0], da, db, %4, q;\n"
       "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
       : "memory");
 }
@@ -112,6 +116,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
       : "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 // Shared-memory matrix descriptor: K-major operand, 128-byte swizzle, rows of
@@ -126,6 +136,15 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr) {
   d |= (uint64_t)1 << 46;
   d |= (uint64_t)2 << 61;
   return d;
+}
+
+// umma_commit for a whole converged warp whose elected lane issued the MMAs
+__device__ __forceinline__ void umma_commit_elected(uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar)
+      : "memory");
 }
 
 // ---------------------------------------------------------------- CTA pairs (cta_group::2)
@@ -215,29 +234,30 @@ __device__ __forceinline__ void umma_i8_kblock_pair(uint32_t d_tmem, uint32_t a_
                                                uint32_t idesc, uint32_t accumulate_first) {
   asm volatile(
       "{\n"
-      ".reg .pred p, q;\n"
+      ".reg .pred e, p, q;\n"
       ".reg .b32 ta, tb;\n"
       ".reg .b64 da, db;\n"
+      "elect.sync _|e, 0xffffffff;\n"
       "setp.ne.b32 p, %5, 0;\n"
-      "setp.ne.b32 q, %4, 0;\n"
+      "setp.ne.b32 q, %4, 0;\n"          // the instruction descriptor is never zero: q = true
       "mov.b64 da, {%1, %3};\n"
       "mov.b64 db, {%2, %3};\n"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, p;\n"
+      "@e tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, p;\n"
       "add.u32 ta, %1, 2;\n"
       "add.u32 tb, %2, 2;\n"
       "mov.b64 da, {ta, %3};\n"
       "mov.b64 db, {tb, %3};\n"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
+      "@e tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
       "add.u32 ta, %1, 4;\n"
       "add.u32 tb, %2, 4;\n"
       "mov.b64 da, {ta, %3};\n"
       "mov.b64 db, {tb, %3};\n"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
+      "@e tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
       "add.u32 ta, %1, 6;\n"
       "add.u32 tb, %2, 6;\n"
       "mov.b64 da, {ta, %3};\n"
       "mov.b64 db, {tb, %3};\n"
-      "tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
+      "@e tcgen05.mma.cta_group::2.kind::i8 [%0], da, db, %4, q;\n"
       "}\n" ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "r"(accumulate_first)
       : "memory");
 }
@@ -245,6 +265,16 @@ __device__ __forceinline__ void umma_i8_kblock_pair(uint32_t d_tmem, uint32_t a_
 // MMA issued so far by this thread has completed
 __device__ __forceinline__ void umma_commit_pair(uint32_t cbar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(cbar) : "memory");
+}
+
+// The same by the elected lane of a converged warp, on the barrier at this offset in both CTAs of the pair.
+__device__ __forceinline__ void umma_commit_both_elected(uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred e;\n.reg .b16 both;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "mov.b16 both, 3;\n"
+      "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n}" ::"r"(bar)
+      : "memory");
 }
 
 }  // namespace smith

@@ -88,27 +88,38 @@ __device__ __forceinline__ void put(__half* at, float v) { __stcs(at, __float2ha
 // tokens' in shared memory.  `at` is the first token's place in C where rows are in order.  (Eight at a
 // time in a loop: code that runs once or twice per launch is paid for by its length.  Unrolled to 32 tokens
 // the epilogue of a small product took 3 us.)
-template <typename T, bool ORDERED>
-__device__ __forceinline__ void store_tokens(const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw, T* column,
-                                             T* at, int64_t ldc, bool mine) {
+template <typename T, bool ORDERED, bool FULL>
+__device__ __forceinline__ void store_eight(const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw, T* column,
+                                            T* at, int64_t ldc, bool mine) {
+  uint64_t sw2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(sw2) : "f"(sw));
 #pragma unroll
   for (int i = 0; i < 8; i += 4) {
-    const float4 s4 = *reinterpret_cast<const float4*>(sa + i);
-    const float s[4] = {s4.x, s4.y, s4.z, s4.w};
+    const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(sa + i);
     int4 t4 = make_int4(0, 0, 0, 0);
     if (!ORDERED) t4 = *reinterpret_cast<const int4*>(to + i);
     const int t[4] = {t4.x, t4.y, t4.z, t4.w};
+    float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      const float v = (float)(int)r[i + j] * s[j] * sw;
-      if (ORDERED) {
-        if (mine && i + j < count) put(at, v);
-        at += ldc;
-      } else if (mine && i + j < count && t[j] >= 0) {
-        put(column + t[j] * ldc, v);
+    for (int j = 0; j < 4; j += 2)      // two tokens to an instruction, each rounded as by itself
+      asm("{\n.reg .b64 t;\nmov.b64 t, {%2, %3};\nmul.rn.f32x2 t, t, %4;\nmul.rn.f32x2 t, t, %5;\nmov.b64 {%0, %1}, t;\n}"
+          : "=f"(v[j]), "=f"(v[j + 1])
+          : "f"((float)(int)r[i + j]), "f"((float)(int)r[i + j + 1]), "l"(j ? s4.y : s4.x), "l"(sw2));
+    if (mine) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        if (!FULL && i + j >= count) break;
+        if (ORDERED) put(at + (i + j) * ldc, v[j]);
+        else if (t[j] >= 0) put(column + t[j] * ldc, v[j]);
       }
     }
   }
+}
+template <typename T, bool ORDERED>
+__device__ __forceinline__ void store_tokens(const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw, T* column,
+                                             T* at, int64_t ldc, bool mine) {
+  if (count >= 8) store_eight<T, ORDERED, true>(r, count, sa, to, sw, column, at, ldc, mine);
+  else store_eight<T, ORDERED, false>(r, count, sa, to, sw, column, at, ldc, mine);
 }
 
 // The same where a scale is outside the plain range; rare, so kept out of line.
@@ -474,11 +485,15 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
       }
       if (store && nt < p.n_tiles) {
         int64_t at = (int64_t)(tile.row0 + c0) * p.ldc + n;
+        uint32_t next[8];
+        tmem_ld8(acc + (uint32_t)c0, next);
 #pragma unroll 1
         for (int c = c0; c < c1; c += 8) {
           uint32_t r[8];
-          tmem_ld8(acc + (uint32_t)c, r);
           tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 8; i++) r[i] = next[i];
+          if (c + 8 < c1) tmem_ld8(acc + (uint32_t)c + 8u, next);       // on its way while these are stored
           if (!alone) join(p, r, c, PAIR ? 2 : 1, (int)rank, worker, w0, others, ch);
           const float* sa = tok_sa + (c - c0);
           const int* to = tok_to + (c - c0);

@@ -205,15 +205,15 @@ __device__ __forceinline__ void make_codes(const uint4& raw, const Coder& coder,
 // A place outside [0, places) is skipped.  Each thread keeps its first HELD vectors in registers; what a
 // longer row has beyond is read again.
 //
-// Two forms.  Many rows are bound by reading them and by instructions (about six per value): 256 threads
-// and 8 vectors in flight each.  Rows fewer than SMs are bound by latency: 512 threads with 2 vectors each
+// Two forms.  Many rows are bound by reading them and by instructions (about six per value): four vectors
+// in flight per thread, as many threads as that takes.  Rows fewer than SMs are bound by latency: 512 threads with 2 vectors each
 // are through soonest (one row of 4096 f32: 128 threads 5.6 us until the product could begin, 256 threads
 // 3.1 us), and with at most 32 registers a thread, so that a block of the product finds room beside (a
 // quarter of an SM's register file holds three of its ten warps; with more registers here, the SMs that
 // hold one of these blocks began the product 2.5 to 5 us late).
 constexpr int kNearPlaces = 32;
 template <typename T, bool WIDE, int HELD, int THREADS>
-__global__ void __launch_bounds__(THREADS, HELD == 2 ? 4 : 1) int8_rows_kernel(const T* a, int64_t lda, int K, int kp, const int* position, int fan,
+__global__ void __launch_bounds__(THREADS, HELD == 2 ? 4 : 2) int8_rows_kernel(const T* a, int64_t lda, int K, int kp, const int* position, int fan,
                                                         int places, uint8_t* codes, float* maxima, int* counters, int n_counters) {
   constexpr int kVec = 16 / sizeof(T);
   // Wait first, then let the product start: what precedes this launch is finished by then, so the
@@ -309,13 +309,13 @@ cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda
   const bool few = rows < device_sm_count();
   const int64_t vecs = (kp * es + 15) / 16;
   int threads = 64;
-  while (threads < (few ? 512 : 256) && threads * (few ? 2 : 4) < vecs) threads *= 2;
+  while (threads < 512 && threads * (few ? 2 : 4) < vecs) threads *= 2;
   using Kernel = void (*)(const void*, int64_t, int, int, const int*, int, int, uint8_t*, float*, int*, int);
   static const Kernel kernels[8] = {
-      (Kernel)int8_rows_kernel<float, false, 8, 256>,  (Kernel)int8_rows_kernel<float, false, 2, 512>,
-      (Kernel)int8_rows_kernel<float, true, 8, 256>,   (Kernel)int8_rows_kernel<float, true, 2, 512>,
-      (Kernel)int8_rows_kernel<__half, false, 8, 256>, (Kernel)int8_rows_kernel<__half, false, 2, 512>,
-      (Kernel)int8_rows_kernel<__half, true, 8, 256>,  (Kernel)int8_rows_kernel<__half, true, 2, 512>};
+      (Kernel)int8_rows_kernel<float, false, 4, 512>,  (Kernel)int8_rows_kernel<float, false, 2, 512>,
+      (Kernel)int8_rows_kernel<float, true, 4, 512>,   (Kernel)int8_rows_kernel<float, true, 2, 512>,
+      (Kernel)int8_rows_kernel<__half, false, 4, 512>, (Kernel)int8_rows_kernel<__half, false, 2, 512>,
+      (Kernel)int8_rows_kernel<__half, true, 4, 512>,  (Kernel)int8_rows_kernel<__half, true, 2, 512>};
   // The product takes nearly all of an SM's shared memory.  These blocks ask for the same split of L1 and
   // shared memory, else an SM might have to drain before it could take a block of the product.
   static PerDeviceFlag configured;

@@ -123,11 +123,13 @@ __device__ __forceinline__ void store_tokens(const uint32_t (&r)[8], int count, 
 }
 
 // The same where a scale is outside the plain range; rare, so kept out of line.
-__device__ __noinline__ void store_odd(const Params& p, const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw,
-                                       float w_max, int row, int n, bool mine) {
+// (The sums come by value: an array handed over by address would live in local memory on every path.)
+__device__ __noinline__ void store_odd(const Params& p, uint4 r0, uint4 r1, int count, const float* sa, const int* to, float sw,
+                                       float w_max, int row, int n) {
+  const uint32_t r[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
   for (int i = 0; i < 8; i++) {
-    if (i >= count || to[i] < 0 || !mine) continue;
+    if (i >= count || to[i] < 0) continue;
     const float a_max = p.a_max[row + i];
     const float v = scaled((int)r[i], sa[i], sw, a_max, w_max);
     if (p.out_f16) put(static_cast<__half*>(p.C) + to[i] * p.ldc + n, v);
@@ -499,7 +501,9 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
           const int* to = tok_to + (c - c0);
           const int count = c1 - c;
           if (!plain) {
-            store_odd(p, r, count, sa, to, sw, w_max, tile.row0 + c, n, mine);
+            if (mine)
+              store_odd(p, make_uint4(r[0], r[1], r[2], r[3]), make_uint4(r[4], r[5], r[6], r[7]), count, sa, to, sw, w_max,
+                        tile.row0 + c, n);
           } else if (p.out_f16) {
             __half* C = static_cast<__half*>(p.C);
             if (p.order) store_tokens<__half, false>(r, count, sa, to, sw, C + n, C, p.ldc, mine);

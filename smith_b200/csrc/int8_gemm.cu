@@ -56,8 +56,7 @@ struct Params {
   int4* partial;                      // two slots of [BT / 4][128] per CTA
   int* counters;                      // one per epilogue warp of each CTA
   float alone, join_fixed, join_each; // see Costs
-  int64_t ldc;
-  int rows, N, experts;
+  int ldc, rows, N, experts;
   int n_tiles, k_slabs;
   int w_tiles;                        // n_tiles, in pairs for the pair form
   int BT;                             // tokens per tile
@@ -84,56 +83,95 @@ __device__ __noinline__ float scaled(int sum, float sa, float sw, float a_max, f
 __device__ __forceinline__ void put(float* at, float v) { __stcs(at, v); }
 __device__ __forceinline__ void put(__half* at, float v) { __stcs(at, __float2half_rn(v)); }
 
-// Eight tokens of one channel: sums r scaled and stored; sa and to (row of C, negative: none) are the
-// tokens' in shared memory.  `at` is the first token's place in C where rows are in order.  (Eight at a
-// time in a loop: code that runs once or twice per launch is paid for by its length.  Unrolled to 32 tokens
-// the epilogue of a small product took 3 us.)
-template <typename T, bool ORDERED, bool FULL>
-__device__ __forceinline__ void store_eight(const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw, T* column,
-                                            T* at, int64_t ldc, bool mine) {
-  uint64_t sw2;
-  asm("mov.b64 %0, {%1, %1};" : "=l"(sw2) : "f"(sw));
+// A tile's workers: w0 .. w0 + others, `worker` this one; CTAs per worker and this CTA's rank among them.
+struct Sharers {
+  int w0, others, worker, ctas, rank;
+};
+
+// Adds the partial sums of a tile's other workers to eight tokens.
+__device__ __forceinline__ void join(const Params& p, uint32_t (&r)[8], int c, const Sharers& o, int ch) {
+#pragma unroll 4
+  for (int k = 0; k < o.others; k++) {
+    const int w = o.w0 + k + (o.w0 + k >= o.worker ? 1 : 0);
+    const int4* slot = p.partial + ((size_t)(o.ctas * w + o.rank) * 2 + (w == o.w0 ? 1 : 0)) * (p.BT * 32) + (c >> 2) * 128 + ch;
 #pragma unroll
-  for (int i = 0; i < 8; i += 4) {
-    const ulonglong2 s4 = *reinterpret_cast<const ulonglong2*>(sa + i);
-    int4 t4 = make_int4(0, 0, 0, 0);
-    if (!ORDERED) t4 = *reinterpret_cast<const int4*>(to + i);
-    const int t[4] = {t4.x, t4.y, t4.z, t4.w};
-    float v[4];
-#pragma unroll
-    for (int j = 0; j < 4; j += 2)      // two tokens to an instruction, each rounded as by itself
-      asm("{\n.reg .b64 t;\nmov.b64 t, {%2, %3};\nmul.rn.f32x2 t, t, %4;\nmul.rn.f32x2 t, t, %5;\nmov.b64 {%0, %1}, t;\n}"
-          : "=f"(v[j]), "=f"(v[j + 1])
-          : "f"((float)(int)r[i + j]), "f"((float)(int)r[i + j + 1]), "l"(j ? s4.y : s4.x), "l"(sw2));
-    if (mine) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (!FULL && i + j >= count) break;
-        if (ORDERED) put(at + (i + j) * ldc, v[j]);
-        else if (t[j] >= 0) put(column + t[j] * ldc, v[j]);
-      }
+    for (int i = 0; i < 2; i++) {
+      const int4 v = __ldcg(&slot[i * 128]);
+      r[4 * i] += (uint32_t)v.x, r[4 * i + 1] += (uint32_t)v.y, r[4 * i + 2] += (uint32_t)v.z, r[4 * i + 3] += (uint32_t)v.w;
     }
   }
 }
-template <typename T, bool ORDERED>
-__device__ __forceinline__ void store_tokens(const uint32_t (&r)[8], int count, const float* sa, const int* to, float sw, T* column,
-                                             T* at, int64_t ldc, bool mine) {
-  if (count >= 8) store_eight<T, ORDERED, true>(r, count, sa, to, sw, column, at, ldc, mine);
-  else store_eight<T, ORDERED, false>(r, count, sa, to, sw, column, at, ldc, mine);
+
+// Tokens [c0, c1) of one channel (lane): sums read from tensor memory, the other workers' added (JOIN), scaled
+// and stored.  sa and to (row of C; negative: none) are the tokens' in shared memory, from c0 on; `column` is
+// the channel's element in row 0 of C (ORDERED: in the row of token c0).  Eight at a time with the next
+// eight and their scales on their way.  The loop is short on purpose: the code of a small product runs once
+// per launch and is paid for by its length (unrolled to 32 tokens it took 3 us), and with two warps per
+// scheduler only loads ahead hide latency.
+template <typename T, bool ORDERED, bool JOIN>
+__device__ __forceinline__ void write_tokens(const Params& p, uint32_t acc, int c0, int c1, const float* sa, const int* to, float sw,
+                                             T* column, bool mine, const Sharers& o, int ch) {
+  uint64_t sw2;
+  asm("mov.b64 %0, {%1, %1};" : "=l"(sw2) : "f"(sw));
+  const int ldc = p.ldc;
+  uint32_t next[8];
+  tmem_ld8(acc + (uint32_t)c0, next);
+  ulonglong2 sa0 = *reinterpret_cast<const ulonglong2*>(sa), sa1 = *reinterpret_cast<const ulonglong2*>(sa + 4);
+  T* at = column;
+#pragma unroll 1
+  for (int c = c0; c < c1; c += 8) {
+    uint32_t r[8];
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; i++) r[i] = next[i];
+    const uint64_t s[4] = {sa0.x, sa0.y, sa1.x, sa1.y};
+    if (c + 8 < c1) {
+      tmem_ld8(acc + (uint32_t)c + 8u, next);
+      sa += 8;
+      sa0 = *reinterpret_cast<const ulonglong2*>(sa), sa1 = *reinterpret_cast<const ulonglong2*>(sa + 4);
+    }
+    if (JOIN) join(p, r, c, o, ch);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)      // two tokens to an instruction, each rounded as by itself
+      asm("{\n.reg .b64 t;\nmov.b64 t, {%2, %3};\nmul.rn.f32x2 t, t, %4;\nmul.rn.f32x2 t, t, %5;\nmov.b64 {%0, %1}, t;\n}"
+          : "=f"(v[j]), "=f"(v[j + 1])
+          : "f"((float)(int)r[j]), "f"((float)(int)r[j + 1]), "l"(s[j / 2]), "l"(sw2));
+    if (mine) {
+      const int count = c1 - c;
+      if (ORDERED && count >= 8) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) put(at + (int64_t)ldc * j, v[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          if (j >= count) break;
+          if (ORDERED) put(at + (int64_t)ldc * j, v[j]);
+          else if (to[j] >= 0) put(column + (int64_t)ldc * to[j], v[j]);
+        }
+      }
+    }
+    if (ORDERED) at += (int64_t)ldc * 8;
+    to += 8;
+  }
 }
 
-// The same where a scale is outside the plain range; rare, so kept out of line.
-// (The sums come by value: an array handed over by address would live in local memory on every path.)
-__device__ __noinline__ void store_odd(const Params& p, uint4 r0, uint4 r1, int count, const float* sa, const int* to, float sw,
-                                       float w_max, int row, int n) {
-  const uint32_t r[8] = {r0.x, r0.y, r0.z, r0.w, r1.x, r1.y, r1.z, r1.w};
+// The same for a tile with a scale outside the plain range; rare, so kept out of line.
+__device__ __noinline__ void write_odd(const Params& p, uint32_t acc, int c0, int c1, const float* sa, const int* to, float sw,
+                                       float w_max, int row, int n, bool mine, bool joined, Sharers o, int ch) {
+  for (int c = c0; c < c1; c += 8) {
+    uint32_t r[8];
+    tmem_ld8(acc + (uint32_t)c, r);
+    tmem_ld_wait();
+    if (joined) join(p, r, c, o, ch);
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    if (i >= count || to[i] < 0) continue;
-    const float a_max = p.a_max[row + i];
-    const float v = scaled((int)r[i], sa[i], sw, a_max, w_max);
-    if (p.out_f16) put(static_cast<__half*>(p.C) + to[i] * p.ldc + n, v);
-    else put(static_cast<float*>(p.C) + to[i] * p.ldc + n, v);
+    for (int j = 0; j < 8; j++) {
+      const int i = c - c0 + j;
+      if (c + j >= c1 || to[i] < 0 || !mine) continue;
+      const float v = scaled((int)r[j], sa[i], sw, p.a_max[row + i], w_max);
+      if (p.out_f16) put(static_cast<__half*>(p.C) + (int64_t)p.ldc * to[i] + n, v);
+      else put(static_cast<float*>(p.C) + (int64_t)p.ldc * to[i] + n, v);
+    }
   }
 }
 
@@ -222,20 +260,6 @@ __device__ __forceinline__ void plan_groups(const Params& p, int* row_first, int
     t += tiles;
     if (i <= p.experts) row_first[i] = v, tile_first[i] = t;
     tiles = __shfl_sync(0xffffffffu, t, 31);
-  }
-}
-
-// Adds the partial sums of a tile's other workers to eight tokens.
-__device__ __forceinline__ void join(const Params& p, uint32_t (&r)[8], int c, int ctas, int rank, int worker, int w0, int others, int ch) {
-#pragma unroll 4
-  for (int k = 0; k < others; k++) {
-    const int w = w0 + k + (w0 + k >= worker ? 1 : 0);
-    const int4* slot = p.partial + ((size_t)(ctas * w + rank) * 2 + (w == w0 ? 1 : 0)) * (p.BT * 32) + (c >> 2) * 128 + ch;
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      const int4 v = __ldcg(&slot[i * 128]);
-      r[4 * i] += (uint32_t)v.x, r[4 * i + 1] += (uint32_t)v.y, r[4 * i + 2] += (uint32_t)v.z, r[4 * i + 3] += (uint32_t)v.w;
-    }
   }
 }
 
@@ -486,35 +510,20 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
         if (store) __threadfence();
       }
       if (store && nt < p.n_tiles) {
-        int64_t at = (int64_t)(tile.row0 + c0) * p.ldc + n;
-        uint32_t next[8];
-        tmem_ld8(acc + (uint32_t)c0, next);
-#pragma unroll 1
-        for (int c = c0; c < c1; c += 8) {
-          uint32_t r[8];
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 8; i++) r[i] = next[i];
-          if (c + 8 < c1) tmem_ld8(acc + (uint32_t)c + 8u, next);       // on its way while these are stored
-          if (!alone) join(p, r, c, PAIR ? 2 : 1, (int)rank, worker, w0, others, ch);
-          const float* sa = tok_sa + (c - c0);
-          const int* to = tok_to + (c - c0);
-          const int count = c1 - c;
-          if (!plain) {
-            if (mine)
-              store_odd(p, make_uint4(r[0], r[1], r[2], r[3]), make_uint4(r[4], r[5], r[6], r[7]), count, sa, to, sw, w_max,
-                        tile.row0 + c, n);
-          } else if (p.out_f16) {
-            __half* C = static_cast<__half*>(p.C);
-            if (p.order) store_tokens<__half, false>(r, count, sa, to, sw, C + n, C, p.ldc, mine);
-            else store_tokens<__half, true>(r, count, sa, to, sw, C, C + at, p.ldc, mine);
-          } else {
-            float* C = static_cast<float*>(p.C);
-            if (p.order) store_tokens<float, false>(r, count, sa, to, sw, C + n, C, p.ldc, mine);
-            else store_tokens<float, true>(r, count, sa, to, sw, C, C + at, p.ldc, mine);
-          }
-          at += 8 * p.ldc;
-        }
+        const Sharers o{w0, others, worker, PAIR ? 2 : 1, (int)rank};
+        const bool ordered = !p.order;
+        const int64_t first = (ordered ? (int64_t)p.ldc * (tile.row0 + c0) : 0) + n;
+        float* C32 = static_cast<float*>(p.C) + first;
+        __half* C16 = static_cast<__half*>(p.C) + first;
+        if (!plain) write_odd(p, acc, c0, c1, tok_sa, tok_to, sw, w_max, tile.row0 + c0, n, mine, !alone, o, ch);
+        else if (alone && ordered && p.out_f16) write_tokens<__half, true, false>(p, acc, c0, c1, tok_sa, tok_to, sw, C16, mine, o, ch);
+        else if (alone && ordered) write_tokens<float, true, false>(p, acc, c0, c1, tok_sa, tok_to, sw, C32, mine, o, ch);
+        else if (ordered && p.out_f16) write_tokens<__half, true, true>(p, acc, c0, c1, tok_sa, tok_to, sw, C16, mine, o, ch);
+        else if (ordered) write_tokens<float, true, true>(p, acc, c0, c1, tok_sa, tok_to, sw, C32, mine, o, ch);
+        else if (alone && p.out_f16) write_tokens<__half, false, false>(p, acc, c0, c1, tok_sa, tok_to, sw, C16, mine, o, ch);
+        else if (alone) write_tokens<float, false, false>(p, acc, c0, c1, tok_sa, tok_to, sw, C32, mine, o, ch);
+        else if (p.out_f16) write_tokens<__half, false, true>(p, acc, c0, c1, tok_sa, tok_to, sw, C16, mine, o, ch);
+        else write_tokens<float, false, true>(p, acc, c0, c1, tok_sa, tok_to, sw, C32, mine, o, ch);
       }
       tc_fence_before();
       __syncwarp();
@@ -659,7 +668,7 @@ cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s) {
   const Costs costs(pl.pair, pl.bt);
   p.alone = (float)costs.alone, p.join_fixed = (float)costs.join_fixed, p.join_each = (float)costs.join_each;
   p.partial = reinterpret_cast<int4*>(codes + pl.codes + pl.maxima + pl.counters);
-  p.offsets = g.offsets, p.order = g.order, p.C = g.C, p.ldc = g.ldc;
+  p.offsets = g.offsets, p.order = g.order, p.C = g.C, p.ldc = (int)g.ldc;
   p.rows = (int)g.rows, p.N = (int)g.N, p.experts = (int)g.experts;
   p.n_tiles = (int)l.n_tiles, p.k_slabs = (int)l.k_slabs, p.BT = pl.bt;
   p.w_tiles = pl.pair ? (p.n_tiles + 1) / 2 : p.n_tiles;

@@ -59,7 +59,8 @@ struct Params {
   int ldc, rows, N, experts;
   int n_tiles, k_slabs;
   int w_tiles;                        // n_tiles, in pairs for the pair form
-  int BT;                             // tokens per tile
+  int BT;                             // most tokens per tile
+  int step;                           // tile sizes are multiples of it: 16, for a pair 32
   int workers;
   int stages, stage_bytes, header, tmem_cols;
   int out_f16;
@@ -233,7 +234,10 @@ struct Walk {
     const int width = min(kBlock, tt - block * kBlock);
     g.nt = in_block / width;
     const int mt = block * kBlock + in_block - g.nt * width;
-    g.expert = e, g.row0 = first + mt * p.BT, g.rows = min(count - mt * p.BT, p.BT);
+    // a group's tiles are of one size (300 rows: 160 and 140, not 256 and 44): a narrow tile moves the same
+    // weights for less work
+    const int size = ((count + tt - 1) / tt + p.step - 1) / p.step * p.step;
+    g.expert = e, g.row0 = first + mt * size, g.rows = min(count - mt * size, size);
     return true;
   }
 };
@@ -286,11 +290,11 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
   const uint32_t rank = PAIR ? cluster_ctarank() : 0u;    // 0: the CTA that issues the pair's MMAs
   const int worker = PAIR ? blockIdx.x >> 1 : blockIdx.x;
 
-  if (tid == 64) {
-    for (int s = 0; s < kMaxStages; s++) mbar_init(smem_u32(&full[s]), PAIR ? 2 : 1), mbar_init(smem_u32(&empty[s]), 1);
-    for (int b = 0; b < 2; b++) mbar_init(smem_u32(&acc_full[b]), 1), mbar_init(smem_u32(&acc_empty[b]), (PAIR ? 2 : 1) * kEpiWarps);
-    mbar_init(smem_u32(drain), 1);
-    *abort_flag = 0;
+  if (warp == 2) {                       // a lane per barrier
+    if (lane < kMaxStages) mbar_init(smem_u32(&full[lane]), PAIR ? 2 : 1), mbar_init(smem_u32(&empty[lane]), 1);
+    else if (lane < kMaxStages + 2) mbar_init(smem_u32(&acc_full[lane - kMaxStages]), 1);
+    else if (lane < kMaxStages + 4) mbar_init(smem_u32(&acc_empty[lane - kMaxStages - 2]), (PAIR ? 2 : 1) * kEpiWarps);
+    else if (lane == kMaxStages + 4) mbar_init(smem_u32(drain), 1), *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
@@ -303,10 +307,15 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
     }
   }
   if (warp == 0) {
+    if (p.offsets) {
 #pragma unroll 4
-    for (int i = lane; i <= p.experts; i += 32) row_first[i] = p.offsets ? min(max(p.offsets[i], 0), p.rows) : (i ? p.rows : 0);
-    __syncwarp();
-    plan_groups(p, row_first, tile_first, lane);
+      for (int i = lane; i <= p.experts; i += 32) row_first[i] = min(max(p.offsets[i], 0), p.rows);
+      __syncwarp();
+      plan_groups(p, row_first, tile_first, lane);
+    } else if (lane == 0) {
+      row_first[0] = 0, row_first[1] = p.rows;
+      tile_first[0] = 0, tile_first[1] = p.w_tiles * ((p.rows + p.BT - 1) / p.BT);
+    }
     __syncwarp();
     // What is left after the full waves: whole tiles (lane 0), l + 1 workers per tile (lane l), or runs of
     // units over all workers (lane 31), whichever is done first.  A worker alone moves its units faster
@@ -351,47 +360,49 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
   const uint32_t ring = smem_u32(tiles);
 
   if (warp == 0) {
-    // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      int s = 0;
-      uint32_t par = 0;
-      int64_t issued = 0;
-      bool ok = true;
-      // The weights of the first ring are on their way before the codes exist (the launch that makes them
-      // lets this one start when all that came before it is done, so weights and group lists are final).
-      for (int pass = 0; pass < 2; pass++) {
-        if (pass) asm volatile("griddepcontrol.wait;" ::: "memory");    // the codes are the previous launch's
-        s = 0, par = 0, issued = 0;
-        Walk walk(sched);
-        Segment g;
-        while (ok && (pass || issued < p.stages) && walk.next(p, sched, g)) {
-          // a pair's second half of an odd last weight tile repeats the first; its results are not stored
-          const int nt = PAIR ? min(2 * g.nt + (int)rank, p.n_tiles - 1) : g.nt;
-          const int half = PAIR ? ((g.rows + 31) / 32 * 32) / 2 : 0;
-          const int64_t block0 = ((int64_t)g.expert * p.n_tiles + nt) * p.k_slabs;
-          for (int ks = g.ks0; ks < g.ks1 && (pass || issued < p.stages); ks++) {
-            if (issued >= p.stages && !(ok = mbar_wait(smem_u32(&empty[s]), par ^ 1u, abort_flag, p.status))) break;
-            const uint32_t dst = ring + (uint32_t)(s * p.stage_bytes);
-            // pair: both CTAs' bytes are counted on the leader's barrier
-            const uint32_t bar = PAIR ? mapa_u32(smem_u32(&full[s]), 0) : smem_u32(&full[s]);
-            if (!pass || issued >= p.stages) {
-              if (PAIR) {
-                mbar_expect_tx_cluster_relaxed(bar, (uint32_t)p.stage_bytes);
-                tma_load_2d_pair(dst, &tmap_w, 0, (int)((block0 + ks) * (kWTile / 1024)), bar);
-              } else {
-                mbar_expect_tx(bar, (uint32_t)p.stage_bytes);
-                bulk_load_plain(dst, p.w + (size_t)(block0 + ks) * kWTile, kWTile, bar);
-              }
+    // ------------------------------------------------------------ producer (the whole warp; one lane issues)
+    int s = 0;
+    uint32_t par = 0;
+    int64_t issued = 0;
+    bool ok = true;
+    const uint32_t bytes = (uint32_t)p.stage_bytes;
+    // pair: both CTAs' bytes are counted on the leader's barriers
+    const uint32_t bar0 = PAIR ? mapa_u32(smem_u32(full), 0) : smem_u32(full);
+    // The weights of the first ring are on their way before the codes exist (the launch that makes them
+    // lets this one start when all that came before it is done, so weights and group lists are final).
+    for (int pass = 0; pass < 2; pass++) {
+      if (pass) asm volatile("griddepcontrol.wait;" ::: "memory");    // the codes are the previous launch's
+      s = 0, par = 0, issued = 0;
+      Walk walk(sched);
+      Segment g;
+      while (ok && (pass || issued < p.stages) && walk.next(p, sched, g)) {
+        // a pair's second half of an odd last weight tile repeats the first; its results are not stored
+        const int nt = PAIR ? min(2 * g.nt + (int)rank, p.n_tiles - 1) : g.nt;
+        const int64_t block0 = ((int64_t)g.expert * p.n_tiles + nt) * p.k_slabs;
+        const int row = g.row0 + (PAIR ? (int)rank * (((g.rows + 31) / 32 * 32) / 2) : 0);
+        for (int ks = g.ks0; ks < g.ks1 && (pass || issued < p.stages); ks++) {
+          if (issued >= p.stages) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[s]), par ^ 1u, abort_flag, p.status));
+          if (!ok) break;
+          const uint32_t dst = ring + (uint32_t)s * bytes, bar = bar0 + (uint32_t)s * 8u;
+          if (!pass || issued >= p.stages) {
+            if (PAIR) {
+              mbar_expect_tx_cluster_elected(bar, bytes);
+              tma_load_2d_pair_elected(dst, &tmap_w, 0, (int)((block0 + ks) * (kWTile / 1024)), bar);
+            } else {
+              mbar_expect_tx_elected(bar, bytes);
+              bulk_load_elected(dst, p.w + (size_t)(block0 + ks) * kWTile, kWTile, bar);
             }
-            if (pass) {   // boxes beyond the last row are filled with zeros and count their bytes all the same
-              if (PAIR) tma_load_2d_pair(dst + kWTile, &tmap_a, ks * 128, g.row0 + (int)rank * half, bar);
-              else tma_load_2d(dst + kWTile, &tmap_a, ks * 128, g.row0, bar);
-            }
-            issued++;
-            if (++s == p.stages) s = 0, par ^= 1u;
           }
+          if (pass) {   // a box beyond the last row is filled with zeros and counts its bytes all the same
+            if (PAIR) tma_load_2d_pair_elected(dst + kWTile, &tmap_a, ks * 128, row, bar);
+            else tma_load_2d_elected(dst + kWTile, &tmap_a, ks * 128, row, bar);
+          }
+          issued++;
+          if (++s == p.stages) s = 0, par ^= 1u;
         }
       }
+    }
+    if (lane == 0) {
       if (*abort_flag && rank == 0) {
         // copies in flight must land before the shared memory goes (the peer's count on these barriers too)
         for (int64_t i = issued > p.stages ? issued - p.stages : 0; i < issued; i++)
@@ -573,7 +584,7 @@ size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 // for a shared tile (writing, the counter, the stores), and for the sums of each other worker.
 struct Costs {
   double alone, join_fixed, join_each;
-  Costs(bool pair, int bt) : alone(pair ? 1.0 : 0.75), join_fixed(pair ? 11.0 : 4.0 + 3.0 * bt / 128), join_each(pair ? 7.0 : 0.5 + 2.0 * bt / 128) {}
+  Costs(bool pair, int bt) : alone(pair ? 1.0 : 0.8), join_fixed(pair ? 11.0 : 4.0 + 3.0 * bt / 128), join_each(pair ? 7.0 : 0.5 + 2.0 * bt / 128) {}
 };
 
 struct Plan {
@@ -659,7 +670,8 @@ cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s) {
 
   CUtensorMap map_a{}, map_w{};
   const int64_t blocks = l.experts * l.n_tiles * l.k_slabs;
-  if (!encode_codes(&map_a, codes, kp, g.rows, pl.pair ? pl.bt / 2 : pl.bt)) return cudaErrorInvalidValue;
+  const int box = pl.pair ? pl.bt / 2 : pl.bt;              // token codes a CTA stages per unit
+  if (!encode_codes(&map_a, codes, kp, g.rows, box)) return cudaErrorInvalidValue;
   if (pl.pair && (blocks * kBlockLines > 0x7FFFFFFF || !encode_blocks(&map_w, g.W, blocks))) return cudaErrorInvalidValue;
   Params p{};
   p.w = static_cast<const uint8_t*>(g.W);
@@ -674,7 +686,8 @@ cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s) {
   p.w_tiles = pl.pair ? (p.n_tiles + 1) / 2 : p.n_tiles;
   p.workers = pl.pair ? pl.ctas / 2 : pl.ctas;
   p.header = (int)align_up(kHeader + (size_t)(g.experts + 1) * 8, 1024);
-  p.stage_bytes = kWTile + (pl.pair ? pl.bt / 2 : pl.bt) * 128;
+  p.step = pl.pair ? 32 : 16;
+  p.stage_bytes = kWTile + box * 128;
   p.stages = (227 * 1024 - p.header) / p.stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
   p.tmem_cols = 64;                                        // a power of two; reads go in chunks of 32 columns

@@ -177,11 +177,6 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cbar) {
 __device__ __forceinline__ void mbar_expect_tx_cluster(uint32_t cbar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cbar), "r"(bytes) : "memory");
 }
-// The same without release semantics, for a thread that publishes nothing but the byte count: a release at
-// cluster scope makes the thread wait for its earlier operations, about 0.6 us per arrival.
-__device__ __forceinline__ void mbar_expect_tx_cluster_relaxed(uint32_t cbar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(cbar), "r"(bytes) : "memory");
-}
 // tensor-map load into this CTA's shared memory whose bytes are counted on a barrier that may live in the peer CTA
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t cbar) {
   asm volatile(
@@ -274,6 +269,44 @@ __device__ __forceinline__ void umma_commit_both_elected(uint32_t bar) {
       "elect.sync _|e, 0xffffffff;\n"
       "mov.b16 both, 3;\n"
       "@e tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n}" ::"r"(bar)
+      : "memory");
+}
+
+// A stage of the pair form, for a whole converged warp: the elected lane announces `bytes` on the barrier
+// (either CTA's, by its shared::cluster address).  Relaxed: the lane publishes nothing but the count, and a
+// release at cluster scope would make it wait for its earlier operations, about 0.6 us per arrival.
+__device__ __forceinline__ void mbar_expect_tx_cluster_elected(uint32_t cbar, uint32_t bytes) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;\n}" ::"r"(cbar), "r"(bytes)
+      : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx_elected(uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}" ::"r"(bar), "r"(bytes)
+      : "memory");
+}
+// Loads issued by the elected lane of a converged warp (tma_load_2d, tma_load_2d_pair, bulk_load_plain).
+__device__ __forceinline__ void tma_load_2d_elected(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair_elected(uint32_t dst, const CUtensorMap* map, int c0, int c1, uint32_t cbar) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4}], [%2];\n}"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(cbar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_load_elected(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "{\n.reg .pred e;\nelect.sync _|e, 0xffffffff;\n"
+      "@e cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n}"
+      ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
       : "memory");
 }
 

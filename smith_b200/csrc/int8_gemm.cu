@@ -19,7 +19,9 @@
 // a slot of scratch and count themselves on a counter (zeroed by the launch that makes the codes).  Whole
 // numbers add in any order, so the result does not depend on which one is last, and nobody waits.
 //
-//   warp 0     producer: one copy of the packed 16 KB weight block and one box of token codes per unit
+//   warp 0     weight producer: one copy of a packed 16 KB block per unit
+//   warp 10    token producer: one box of codes per unit (one warp for both took 480 clocks per unit, as long
+//              as the MMAs of a 256-token tile take)
 //   warp 1     MMA issuer; two accumulators in tensor memory, so the next tile runs during an epilogue
 //   warps 2-9  epilogue: two warps share a quarter of the lanes, each takes half of the tile's tokens
 // Every mbarrier wait is time-bounded (pipeline.cuh); on a give-up the CTA waits (bounded) for its copies
@@ -38,7 +40,8 @@ namespace smith {
 namespace {
 
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = (2 + kEpiWarps) * 32;
+constexpr int kTokenWarp = 2 + kEpiWarps;
+constexpr int kThreads = (kTokenWarp + 1) * 32;
 constexpr int kWTile = 16384;         // 128 channels x 128 k
 constexpr int kMaxStages = 12;
 constexpr int kWarpTokens = 128;      // most tokens of one epilogue warp: half of a tile
@@ -267,6 +270,33 @@ __device__ __forceinline__ void plan_groups(const Params& p, int* row_first, int
   }
 }
 
+// The stages of a ring as one warp goes through them.  After step() the next stage's barrier is looked at
+// while the warp issues what belongs to this one; wait() then often finds the answer there.
+struct Ring {
+  uint32_t bars;            // 8 bytes each
+  int stages, s = 0;
+  uint32_t par;             // phase parity that wait() expects
+  bool seen = false;
+  __device__ Ring(uint32_t bars, int stages, uint32_t par) : bars(bars), stages(stages), par(par) {}
+  __device__ __forceinline__ bool wait(volatile int* abort_flag, int* status) {
+    return seen || __all_sync(0xffffffffu, mbar_wait(bars + 8u * s, par, abort_flag, status));
+  }
+  __device__ __forceinline__ bool look() const {        // at the stage after this one
+    const bool wrap = s + 1 == stages;
+    return mbar_test(bars + (wrap ? 0u : 8u * (s + 1)), par ^ (wrap ? 1u : 0u));
+  }
+  __device__ __forceinline__ void step(bool looked) {
+    seen = __all_sync(0xffffffffu, looked);
+    if (++s == stages) s = 0, par ^= 1u;
+  }
+};
+
+// Bounded time for copies in flight to land after a give-up, before the shared memory goes.
+__device__ __forceinline__ void let_copies_land() {
+  const long long t0 = clock64();
+  while (clock64() - t0 < 400000) {}                       // about 0.2 ms
+}
+
 template <bool PAIR>
 __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
                                                                 const __grid_constant__ CUtensorMap tmap_w,
@@ -360,63 +390,65 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
   const uint32_t ring = smem_u32(tiles);
 
   if (warp == 0) {
-    // ------------------------------------------------------------ producer (the whole warp; one lane issues)
-    int s = 0;
-    uint32_t par = 0;
-    int64_t issued = 0;
-    bool ok = true;
+    // ------------------------------------------------------------ weight producer (the whole warp; one lane issues)
+    // Does not wait for the launch that makes the codes: that one lets this one start when all that came
+    // before it is done, so weights and group lists are final.  The first ring is on its way by then.
     const uint32_t bytes = (uint32_t)p.stage_bytes;
     // pair: both CTAs' bytes are counted on the leader's barriers
     const uint32_t bar0 = PAIR ? mapa_u32(smem_u32(full), 0) : smem_u32(full);
-    // The weights of the first ring are on their way before the codes exist (the launch that makes them
-    // lets this one start when all that came before it is done, so weights and group lists are final).
-    for (int pass = 0; pass < 2; pass++) {
-      if (pass) asm volatile("griddepcontrol.wait;" ::: "memory");    // the codes are the previous launch's
-      s = 0, par = 0, issued = 0;
-      Walk walk(sched);
-      Segment g;
-      while (ok && (pass || issued < p.stages) && walk.next(p, sched, g)) {
-        // a pair's second half of an odd last weight tile repeats the first; its results are not stored
-        const int nt = PAIR ? min(2 * g.nt + (int)rank, p.n_tiles - 1) : g.nt;
-        const int64_t block0 = ((int64_t)g.expert * p.n_tiles + nt) * p.k_slabs;
-        const int row = g.row0 + (PAIR ? (int)rank * (((g.rows + 31) / 32 * 32) / 2) : 0);
-        for (int ks = g.ks0; ks < g.ks1 && (pass || issued < p.stages); ks++) {
-          if (issued >= p.stages) ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[s]), par ^ 1u, abort_flag, p.status));
-          if (!ok) break;
-          const uint32_t dst = ring + (uint32_t)s * bytes, bar = bar0 + (uint32_t)s * 8u;
-          if (!pass || issued >= p.stages) {
-            if (PAIR) {
-              mbar_expect_tx_cluster_elected(bar, bytes);
-              tma_load_2d_pair_elected(dst, &tmap_w, 0, (int)((block0 + ks) * (kWTile / 1024)), bar);
-            } else {
-              mbar_expect_tx_elected(bar, bytes);
-              bulk_load_elected(dst, p.w + (size_t)(block0 + ks) * kWTile, kWTile, bar);
-            }
-          }
-          if (pass) {   // a box beyond the last row is filled with zeros and counts its bytes all the same
-            if (PAIR) tma_load_2d_pair_elected(dst + kWTile, &tmap_a, ks * 128, row, bar);
-            else tma_load_2d_elected(dst + kWTile, &tmap_a, ks * 128, row, bar);
-          }
-          issued++;
-          if (++s == p.stages) s = 0, par ^= 1u;
+    Ring r(smem_u32(empty), p.stages, 1u);                 // a fresh barrier is past phase "1": nothing to wait for
+    bool ok = true;
+    Walk walk(sched);
+    Segment g;
+    while (ok && walk.next(p, sched, g)) {
+      // a pair's second half of an odd last weight tile repeats the first; its results are not stored
+      const int nt = PAIR ? min(2 * g.nt + (int)rank, p.n_tiles - 1) : g.nt;
+      const int64_t block0 = ((int64_t)g.expert * p.n_tiles + nt) * p.k_slabs;
+      for (int ks = g.ks0; ks < g.ks1; ks++) {
+        if (!(ok = r.wait(abort_flag, p.status))) break;
+        const bool looked = r.look();
+        const uint32_t dst = ring + (uint32_t)r.s * bytes, bar = bar0 + 8u * r.s;
+        if (PAIR) {
+          mbar_expect_tx_cluster_elected(bar, bytes);
+          tma_load_2d_pair_elected(dst, &tmap_w, 0, (int)((block0 + ks) * (kWTile / 1024)), bar);
+        } else {
+          mbar_expect_tx_elected(bar, bytes);
+          bulk_load_elected(dst, p.w + (size_t)(block0 + ks) * kWTile, kWTile, bar);
         }
+        r.step(looked);
       }
     }
-    if (lane == 0) {
-      if (*abort_flag && rank == 0) {
-        // copies in flight must land before the shared memory goes (the peer's count on these barriers too)
-        for (int64_t i = issued > p.stages ? issued - p.stages : 0; i < issued; i++)
-          for (int spin = 0; spin < 100000 && !mbar_try(smem_u32(&full[i % p.stages]), (uint32_t)(i / p.stages) & 1u); spin++) {}
+    if (!ok) let_copies_land();
+  } else if (warp == kTokenWarp) {
+    // ------------------------------------------------------------ token producer
+    asm volatile("griddepcontrol.wait;" ::: "memory");     // the codes are the previous launch's
+    const uint32_t bytes = (uint32_t)p.stage_bytes;
+    const uint32_t bar0 = PAIR ? mapa_u32(smem_u32(full), 0) : smem_u32(full);
+    Ring r(smem_u32(empty), p.stages, 1u);
+    bool ok = true;
+    Walk walk(sched);
+    Segment g;
+    while (ok && walk.next(p, sched, g)) {
+      const int row = g.row0 + (PAIR ? (int)rank * (((g.rows + 31) / 32 * 32) / 2) : 0);
+      for (int ks = g.ks0; ks < g.ks1; ks++) {
+        if (!(ok = r.wait(abort_flag, p.status))) break;
+        const bool looked = r.look();
+        const uint32_t dst = ring + (uint32_t)r.s * bytes + kWTile, bar = bar0 + 8u * r.s;
+        // a box beyond the last row is filled with zeros and counts its bytes all the same
+        if (PAIR) tma_load_2d_pair_elected(dst, &tmap_a, ks * 128, row, bar);
+        else tma_load_2d_elected(dst, &tmap_a, ks * 128, row, bar);
+        r.step(looked);
       }
     }
+    if (!ok) let_copies_land();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (pair: the leader's only)
     if (rank == 0) {
       const uint64_t desc0 = smem_desc_sw128(ring);
       const uint32_t lo0 = (uint32_t)desc0, hi = (uint32_t)(desc0 >> 32), step = (uint32_t)p.stage_bytes >> 4;
-      int s = 0, seq = 0;
-      uint32_t par = 0, a_lo = lo0;
+      int seq = 0;
       bool ok = true;
+      Ring r(smem_u32(full), p.stages, 0u);
       Walk walk(sched);
       Segment g;
       for (; ok && walk.next(p, sched, g); seq++) {
@@ -429,18 +461,18 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
         tc_fence_after();
         uint32_t first = 0;
         for (int ks = g.ks0; ks < g.ks1; ks++, first = 1) {
-          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), par, abort_flag, p.status));
-          if (!ok) break;
+          if (!(ok = r.wait(abort_flag, p.status))) break;
           tc_fence_after();
+          const bool looked = r.look();
+          const uint32_t a_lo = lo0 + (uint32_t)r.s * step, done = smem_u32(empty) + 8u * r.s;
           if (PAIR) {
             umma_i8_kblock_pair(acc, a_lo, a_lo + (kWTile >> 4), hi, idesc, first);
-            umma_commit_both_elected(smem_u32(&empty[s]));
+            umma_commit_both_elected(done);
           } else {
             umma_i8_kblock(acc, a_lo, a_lo + (kWTile >> 4), hi, idesc, first);
-            umma_commit_elected(smem_u32(&empty[s]));
+            umma_commit_elected(done);
           }
-          a_lo += step;
-          if (++s == p.stages) s = 0, par ^= 1u, a_lo = lo0;
+          r.step(looked);
         }
         if (!ok) break;
         if (PAIR) umma_commit_both_elected(smem_u32(&acc_full[b]));

@@ -35,7 +35,19 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// The same with a suspend-time hint (nanoseconds): the thread may stay suspended that long, and is
+// Whether the phase is over, without waiting.
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n.reg .pred p;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// mbar_try with a suspend-time hint (nanoseconds): the thread may stay suspended that long, and is
 // resumed as soon as the phase completes.  Without the hint a waiting thread comes back after a short
 // system-chosen time and polls again, and the polls of a CTA's waiting warps take issue slots (and
 // power) from the warps that work: a quarter of all instructions of the list kernel were such polls.

@@ -119,16 +119,16 @@ __global__ void __launch_bounds__(256) int8_pack_kernel(const T* __restrict__ w,
 
 // ------------------------------------------------------------------------------------ activations, per product
 // Sixteen bytes of a row from element k: one load, or (rows that do not start on 16 bytes, the row's end)
-// value by value, zeros beyond K.
+// value by value, zeros beyond K.  Through L2: the row may just have been written by the launch before.
 template <typename T, bool WIDE>
 __device__ __forceinline__ uint4 load16(const T* x, int k, int K) {
   constexpr int kVec = 16 / sizeof(T);
-  if (WIDE && k + kVec <= K) return *reinterpret_cast<const uint4*>(x + k);
+  if (WIDE && k + kVec <= K) return __ldcg(reinterpret_cast<const uint4*>(x + k));
   uint32_t w[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     if (sizeof(T) == 4) {
-      w[i] = k + i < K ? reinterpret_cast<const uint32_t*>(x)[k + i] : 0u;
+      w[i] = k + i < K ? __ldcg(reinterpret_cast<const uint32_t*>(x) + k + i) : 0u;
     } else {
       const uint16_t* h = reinterpret_cast<const uint16_t*>(x) + k + 2 * i;
       w[i] = (k + 2 * i < K ? (uint32_t)h[0] : 0u) | (k + 2 * i + 1 < K ? (uint32_t)h[1] << 16 : 0u);
@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(THREADS, HELD == 2 ? 4 : 2) int8_rows_kernel(c
     for (int i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
   __shared__ unsigned warp_most[THREADS / 32];
   __shared__ int near_places[kNearPlaces];   // the row's places, fetched while its values are on their way
-  if (threadIdx.x < kNearPlaces) near_places[threadIdx.x] = !position ? (int)row : threadIdx.x < fan ? position[row * fan + threadIdx.x] : -1;
+  if (threadIdx.x < kNearPlaces) near_places[threadIdx.x] = !position ? (int)row : threadIdx.x < fan ? __ldcg(&position[row * fan + threadIdx.x]) : -1;
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < HELD; i++) take_most<T>(m, held[i]);

@@ -11,13 +11,24 @@
 // tokens its second: a tile takes 16 to 256 tokens, so one token wastes little, and lane = channel lets
 // the epilogue store each token's 32 channels per warp as one contiguous segment without a transpose.
 //
-// One persistent launch.  A tile is 128 channels (a CTA pair: 256) by BT tokens of one group, a unit one
-// slab of 128 k of a tile; tiles are ordered with tokens fastest, then channels, then groups, so weights
-// come from HBM once and the token codes stay in L2.  The units of all tiles are dealt to the workers
-// (CTAs or pairs) in equal contiguous runs where whole tiles would leave workers idle; a tile that two or
-// more workers share is joined by the one that finishes last: the others leave their s32 partial sums in
-// a slot of scratch and count themselves on a counter (zeroed by the launch that makes the codes).  Whole
-// numbers add in any order, so the result does not depend on which one is last, and nobody waits.
+// One persistent launch.  A tile is 128 channels (a CTA pair: 256) by up to BT tokens of one group, a unit
+// one slab of 128 k of a tile.  Full waves of tiles go to the workers (CTAs or pairs) whole, in blocks of
+// neighbouring tiles so that what runs at one time shares its operands.  What is left after them -- often all
+// there is -- is dealt in parts of tiles where that is sooner done.  A tile that two or more workers share is
+// joined by the one that finishes last: the others leave their s32 partial sums in a slot of scratch and
+// count themselves on a counter (zeroed by the launch that makes the codes).  Whole numbers add in any
+// order, so the result does not depend on which one is last, and nobody waits.
+//
+// Bounds, measured on a B200 (whole call, codes included):
+//   4096 x 4096 x 14336 f16   191 us = 2.5 POP/s; the product alone keeps the tensor pipe 81 % busy, at the
+//                             board's power limit (SM clock 1.4 to 1.6 of 1.965 GHz); DRAM 76 MB read, the
+//                             operands once
+//   16 x 4096 x 14336 f32     15 us, 59 MB of weights: HBM, and about 4 us of launch, code and set-up latency
+//   1 x 4096 x 4096 f32       9.6 us: latency (launch and codes 2, set-up 1.3, first weights 1.2, weights 2.6,
+//                             joining 1)
+// What the steps gave: loads announced without release semantics 291 -> 191 us at the largest size; MMAs
+// issued by a converged warp 383 -> 183 clocks per unit; no local memory in the epilogue 264 -> 215 k clocks;
+// weights and codes loaded by separate warps 480 -> 340 clocks per unit.
 //
 //   warp 0     weight producer: one copy of a packed 16 KB block per unit
 //   warp 10    token producer: one box of codes per unit (one warp for both took 480 clocks per unit, as long
@@ -46,7 +57,7 @@ constexpr int kWTile = 16384;         // 128 channels x 128 k
 constexpr int kMaxStages = 12;
 constexpr int kWarpTokens = 128;      // most tokens of one epilogue warp: half of a tile
 constexpr int kHeader = 512 + kEpiWarps * kWarpTokens * 8;        // barriers; the group lists follow
-constexpr int kMinUnits = 2;          // fewest units per worker
+constexpr int kMinUnits = 2;          // fewest units per worker where runs go over tile borders
 constexpr int kBlock = 16;            // token tiles side by side (4096 x 4096 x 14336: 4 -> 202 us, 8 -> 192, 16 -> 188)
 
 struct Params {
@@ -181,7 +192,7 @@ __device__ __noinline__ void write_odd(const Params& p, uint32_t acc, int c0, in
 
 // ---------------------------------------------------------------- the schedule
 // Equal contiguous runs of `total` units over `workers`: the first total % workers runs hold one more.
-// (At most workers - 1 tiles are dealt, so units count below 2^18.)
+// (At most workers - 1 tiles are dealt, so there are fewer than 2^18 units.)
 struct Deal {
   int q, r;
   __device__ Deal(int total, int workers) : q(total / workers), r(total - total / workers * workers) {}
@@ -246,8 +257,8 @@ struct Walk {
 };
 
 // Group boundaries come from device memory: clamped and made to rise, so that nothing they hold leads
-// outside the rows or covers a row twice.  One warp, on row_first as fetched; tiles of a
-// group = weight tiles x token tiles.
+// outside the rows or covers a row twice.  One warp, on row_first as fetched; tiles of a group = weight tiles
+// x token tiles.
 __device__ __forceinline__ void plan_groups(const Params& p, int* row_first, int* tile_first, int lane) {
   int high = 0, tiles = 0;
   if (lane == 0) tile_first[0] = 0;
@@ -292,15 +303,16 @@ struct Ring {
 };
 
 // Bounded time for copies in flight to land after a give-up, before the shared memory goes.
+constexpr long long kLandCycles = 400000;                  // about 0.2 ms
 __device__ __forceinline__ void let_copies_land() {
   const long long t0 = clock64();
-  while (clock64() - t0 < 400000) {}                       // about 0.2 ms
+  while (clock64() - t0 < kLandCycles) {}
 }
 
 template <bool PAIR>
-__global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a,
-                                                                const __grid_constant__ CUtensorMap tmap_w,
-                                                                const __grid_constant__ Params p) {
+__global__ void __maxnreg__(128)       // three warps a scheduler leave room for a block that makes codes (int8_rows.cu)
+int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w,
+                 const __grid_constant__ Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem);     // [kMaxStages] a stage's codes landed
   uint64_t* empty = full + kMaxStages;                     // [kMaxStages] its MMAs are done
@@ -481,7 +493,8 @@ __global__ void __maxnreg__(128) int8_gemm_kernel(const __grid_constant__ CUtens
       if (!ok) {
         if (PAIR) umma_commit_both_elected(smem_u32(drain));
         else umma_commit_elected(smem_u32(drain));
-        for (int spin = 0; spin < 100000 && !mbar_try(smem_u32(drain), 0); spin++) {}
+        const long long t0 = clock64();
+        while (!mbar_try(smem_u32(drain), 0) && clock64() - t0 < kLandCycles) {}
       }
     }
   } else {
@@ -642,7 +655,8 @@ bool make_plan(int64_t rows, int64_t N, int64_t K, int64_t experts, bool groups,
     pl->bt = 256;
     double least = 0;
     const int64_t slabs = (K + 127) / 128, w_tiles = (N + 255) / 256, workers = pl->ctas / 2;
-    for (int64_t tt = (rows + 255) / 256; !groups && tt <= (rows + 127) / 128; tt++) {
+    // (of many waves the last is a small part: the widest tile then)
+    for (int64_t tt = (rows + 255) / 256; !groups && tt <= (rows + 127) / 128 && tt * w_tiles < 16 * workers; tt++) {
       const int bt = (int)(((rows + tt - 1) / tt + 31) / 32 * 32);
       const int64_t tiles = w_tiles * tt, left = tiles % workers;
       const Costs c(true, bt);
@@ -722,7 +736,7 @@ cudaError_t launch_int8_gemm(const Int8Gemm& g, Workspace ws, cudaStream_t s) {
   p.stage_bytes = kWTile + box * 128;
   p.stages = (227 * 1024 - p.header) / p.stage_bytes;
   if (p.stages > kMaxStages) p.stages = kMaxStages;
-  p.tmem_cols = 64;                                        // a power of two; reads go in chunks of 32 columns
+  p.tmem_cols = 32;                                        // a power of two, 32 at least
   while (p.tmem_cols < 2 * pl.bt) p.tmem_cols <<= 1;
   p.out_f16 = g.dtype == kDenseF16;
   // tcgen05.mma kind::i8 instruction descriptor: [4,6) D = s32 (2); [7,10) A and [10,13) B signed 8-bit (1);

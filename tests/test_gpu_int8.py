@@ -54,7 +54,8 @@ def data(seed, M, K, N, dtype, experts=None):
 SHAPES = [(1, 1, 1), (1, 2, 3), (2, 33, 5), (1, 128, 128), (16, 128, 128), (17, 127, 129), (15, 129, 257), (1, 4096, 1024),
           (4, 14336, 136), (8, 640, 4096), (31, 1000, 300), (32, 1024, 512), (33, 384, 640), (63, 100, 1000),
           (64, 2048, 130), (65, 257, 513), (127, 513, 255), (128, 512, 512), (129, 511, 513), (255, 640, 384),
-          (256, 256, 256), (257, 1100, 300), (511, 384, 1000), (513, 2048, 640), (700, 130, 2000), (1031, 900, 777)]
+          (256, 256, 256), (257, 1100, 300), (511, 384, 1000), (513, 2048, 640), (700, 130, 2000), (1031, 900, 777),
+          (200, 20001, 300), (150, 64, 20000), (4097, 128, 128), (2500, 1024, 2500), (16, 14336, 4096), (100, 5000, 24)]
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
@@ -201,7 +202,8 @@ def expected(a_sorted, w, offsets, order=None, fill=np.nan):
 
 GROUPED = [  # tokens, fan, experts, K, N
     (1, 1, 1, 64, 64), (1, 8, 16, 300, 200), (3, 2, 5, 128, 128), (16, 2, 8, 257, 130), (40, 4, 64, 200, 70),
-    (150, 2, 3, 640, 300), (301, 2, 12, 131, 277), (64, 8, 1024, 40, 20), (700, 1, 2, 100, 513), (513, 4, 9, 384, 256)]
+    (150, 2, 3, 640, 300), (301, 2, 12, 131, 277), (64, 8, 1024, 40, 20), (700, 1, 2, 100, 513), (513, 4, 9, 384, 256), (3000, 2, 4, 1300, 520), (40000, 4, 1024, 64, 40),
+    (5, 100, 7, 90, 33), (2, 8, 8, 4096, 1024)]
 
 
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
@@ -382,6 +384,42 @@ def test_captured_graphs_share_scratch_and_outlive_its_growth():
     assert R.same_bits(matmul(big, pack(wbig), 64), want)
     for g in graphs:
         device.graphDestroy(g)
+
+
+def test_two_contexts_at_once():
+    """A second context has a stream and scratch of its own: its calls may run beside the first one's."""
+    import ctypes as C
+    import torch
+    lib = device.lib
+    other = lib.smith_init_device(device.deviceIndex())
+    assert other
+    a, w = data(21, 65, 3000, 500, np.float32)
+    want, packed = R.product(a, w), pack(w)
+    first = DevBuf.of(a), DevBuf(65 * 500 * 4)
+    x = torch.from_numpy(a).cuda()
+    y = torch.zeros(65, 500, device="cuda")
+    torch.cuda.synchronize()
+    handles = [lib.smith_wrap_device_memory(other, C.c_void_p(p), n) for p, n in
+               ((x.data_ptr(), a.nbytes), (device.devicePtr(packed.handle), packed.nbytes), (y.data_ptr(), 65 * 500 * 4))]
+    for _ in range(20):
+        device.int8Matmul(device.DTYPE_F32, first[0].handle, packed.handle, first[1].handle, 65, 500, 3000)
+        assert lib.smith_int8_matmul(other, 0, handles[0], handles[1], handles[2], 65, 500, 3000, 0, 0) == 0
+    device.synchronize()
+    assert lib.smith_synchronize(other) == 0
+    assert R.same_bits(first[1].get(np.float32).reshape(65, 500), want)
+    assert R.same_bits(y.cpu().numpy(), want)
+    for h in handles:
+        lib.smith_release_buffer(h)
+    lib.smith_destroy(other)
+
+
+def test_same_call_gives_the_same_bits_every_time():
+    """Shared tiles are joined by whichever worker is last: whole numbers, so it does not show."""
+    for M, K, N in [(1, 4096, 1024), (24, 9000, 384), (300, 7000, 700)]:
+        a, w = data(M, M, K, N, np.float16)
+        packed, want = pack(w), R.product(a, w)
+        for _ in range(25):
+            assert R.same_bits(matmul(a, packed, N), want)
 
 
 def test_capture_of_a_call_that_needs_more_scratch_is_refused():

@@ -202,19 +202,20 @@ __device__ __forceinline__ void make_codes(const uint4& raw, const Coder& coder,
 
 // One block per row of a: its maximum, then its codes (row-major, rows of kp bytes, zeros from K on) at
 // the row's place, or -- with `position` -- at the `fan` places of the row in a list sorted by expert.
-// A place outside [0, places) is skipped.  Each thread keeps its first HELD vectors in registers; what a
+// A place outside [0, places) is skipped.  Each thread keeps its first kHeld vectors in registers; what a
 // longer row has beyond is read again.
 //
-// Two forms.  Many rows are bound by reading them and by instructions (about six per value): four vectors
-// in flight per thread, as many threads as that takes.  Rows fewer than SMs are bound by latency: 512 threads with 2 vectors each
-// are through soonest (one row of 4096 f32: 128 threads 5.6 us until the product could begin, 256 threads
-// 3.1 us), and with at most 32 registers a thread, so that a block of the product finds room beside (a
-// quarter of an SM's register file holds three of its ten warps; with more registers here, the SMs that
-// hold one of these blocks began the product 2.5 to 5 us late).
-constexpr int kNearPlaces = 32;
-template <typename T, bool WIDE, int HELD, int THREADS>
-__global__ void __launch_bounds__(THREADS, HELD == 2 ? 4 : 2) int8_rows_kernel(const T* a, int64_t lda, int K, int kp, const int* position, int fan,
-                                                        int places, uint8_t* codes, float* maxima, int* counters, int n_counters) {
+// Many rows are bound by reading them and by instructions (about six per value), few by latency: two vectors
+// per thread serve both.  (4096 rows of 4096 f16: 15 us, 3.4 TB/s of reads and writes; four vectors and half
+// the threads 16.  One row of 4096 f32, until the product could begin: 128 threads 5.6 us, 256 threads 3.1,
+// 512 threads 1.5.)  At most 32 registers a thread, so that a block of the product finds room beside: a
+// quarter of an SM's register file holds three of its eleven warps, and with more registers here the SMs
+// that hold one of these blocks began the product 2.5 to 5 us late.
+constexpr int kNearPlaces = 32, kHeld = 2, kMostThreads = 1024;
+template <typename T, bool WIDE>
+__global__ void __launch_bounds__(kMostThreads, 2)
+int8_rows_kernel(const T* a, int64_t lda, int K, int kp, const int* position, int fan, int places, uint8_t* codes, float* maxima,
+                 int* counters, int n_counters) {
   constexpr int kVec = 16 / sizeof(T);
   // Wait first, then let the product start: what precedes this launch is finished by then, so the
   // product may read weights and group boundaries before its own wait.
@@ -223,19 +224,19 @@ __global__ void __launch_bounds__(THREADS, HELD == 2 ? 4 : 2) int8_rows_kernel(c
   const int64_t row = blockIdx.x;
   const T* x = a + row * lda;
   const int first = threadIdx.x * kVec, step = blockDim.x * kVec;
-  uint4 held[HELD];
+  uint4 held[kHeld];
 #pragma unroll
-  for (int i = 0; i < HELD; i++) held[i] = first + i * step < K ? load16<T, WIDE>(x, first + i * step, K) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < kHeld; i++) held[i] = first + i * step < K ? load16<T, WIDE>(x, first + i * step, K) : make_uint4(0, 0, 0, 0);
   if (blockIdx.x == 0)                       // the product's counters of shared tiles start at 0 in every call
     for (int i = threadIdx.x; i < n_counters; i += blockDim.x) counters[i] = 0;
-  __shared__ unsigned warp_most[THREADS / 32];
+  __shared__ unsigned warp_most[kMostThreads / 32];
   __shared__ int near_places[kNearPlaces];   // the row's places, fetched while its values are on their way
   if (threadIdx.x < kNearPlaces) near_places[threadIdx.x] = !position ? (int)row : threadIdx.x < fan ? __ldcg(&position[row * fan + threadIdx.x]) : -1;
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < HELD; i++) take_most<T>(m, held[i]);
+  for (int i = 0; i < kHeld; i++) take_most<T>(m, held[i]);
 #pragma unroll 4
-  for (int k = first + HELD * step; k < K; k += step) take_most<T>(m, load16<T, WIDE>(x, k, K));
+  for (int k = first + kHeld * step; k < K; k += step) take_most<T>(m, load16<T, WIDE>(x, k, K));
   if (sizeof(T) == 2) m = max(m & 0xFFFFu, m >> 16);
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = m;
@@ -261,9 +262,9 @@ __global__ void __launch_bounds__(THREADS, HELD == 2 ? 4 : 2) int8_rows_kernel(c
     }
   };
 #pragma unroll
-  for (int i = 0; i < HELD; i++)
+  for (int i = 0; i < kHeld; i++)
     if (first + i * step < kp) put_codes(first + i * step, held[i]);
-  for (int k = first + HELD * step; k < kp; k += step) put_codes(k, k < K ? load16<T, WIDE>(x, k, K) : make_uint4(0, 0, 0, 0));
+  for (int k = first + kHeld * step; k < kp; k += step) put_codes(k, k < K ? load16<T, WIDE>(x, k, K) : make_uint4(0, 0, 0, 0));
 }
 
 }  // namespace
@@ -306,16 +307,14 @@ cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda
   const int64_t kp = (K + 127) / 128 * 128;
   const int es = dtype == kDenseF16 ? 2 : 4;
   const bool wide = ((reinterpret_cast<uintptr_t>(a) | (uintptr_t)(lda * es)) & 15) == 0;
-  const bool few = rows < device_sm_count();
   const int64_t vecs = (kp * es + 15) / 16;
+  // rows fewer than SMs: at most 512 threads, which fit beside a block of the product
+  const int most_threads = rows < device_sm_count() ? 512 : kMostThreads;
   int threads = 64;
-  while (threads < 512 && threads * (few ? 2 : 4) < vecs) threads *= 2;
+  while (threads < most_threads && threads * kHeld < vecs) threads *= 2;
   using Kernel = void (*)(const void*, int64_t, int, int, const int*, int, int, uint8_t*, float*, int*, int);
-  static const Kernel kernels[8] = {
-      (Kernel)int8_rows_kernel<float, false, 4, 512>,  (Kernel)int8_rows_kernel<float, false, 2, 512>,
-      (Kernel)int8_rows_kernel<float, true, 4, 512>,   (Kernel)int8_rows_kernel<float, true, 2, 512>,
-      (Kernel)int8_rows_kernel<__half, false, 4, 512>, (Kernel)int8_rows_kernel<__half, false, 2, 512>,
-      (Kernel)int8_rows_kernel<__half, true, 4, 512>,  (Kernel)int8_rows_kernel<__half, true, 2, 512>};
+  static const Kernel kernels[4] = {(Kernel)int8_rows_kernel<float, false>, (Kernel)int8_rows_kernel<float, true>,
+                                    (Kernel)int8_rows_kernel<__half, false>, (Kernel)int8_rows_kernel<__half, true>};
   // The product takes nearly all of an SM's shared memory.  These blocks ask for the same split of L1 and
   // shared memory, else an SM might have to drain before it could take a block of the product.
   static PerDeviceFlag configured;
@@ -337,7 +336,7 @@ cudaError_t launch_int8_rows(int dtype, const void* a, int64_t rows, int64_t lda
   count_launch();
   int ikp = (int)kp, iK = (int)K, iplaces = (int)places;
   void* args[] = {&a, &lda, &iK, &ikp, &position, &fan, &iplaces, &codes, &maxima, &counters, &n_counters};
-  return cudaLaunchKernelExC(&cfg, (const void*)kernels[(dtype == kDenseF16 ? 4 : 0) + (wide ? 2 : 0) + (few ? 1 : 0)], args);
+  return cudaLaunchKernelExC(&cfg, (const void*)kernels[(dtype == kDenseF16 ? 2 : 0) + (wide ? 1 : 0)], args);
 }
 
 }  // namespace smith

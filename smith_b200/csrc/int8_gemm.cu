@@ -20,11 +20,11 @@
 // order, so the result does not depend on which one is last, and nobody waits.
 //
 // Bounds, measured on a B200 (whole call, codes included):
-//   4096 x 4096 x 14336 f16   191 us = 2.5 POP/s; the product alone keeps the tensor pipe 81 % busy, at the
+//   4096 x 4096 x 14336 f16   189 us = 2.5 POP/s; the product alone keeps the tensor pipe 81 % busy, at the
 //                             board's power limit (SM clock 1.4 to 1.6 of 1.965 GHz); DRAM 76 MB read, the
 //                             operands once
 //   16 x 4096 x 14336 f32     15 us, 59 MB of weights: HBM, and about 4 us of launch, code and set-up latency
-//   1 x 4096 x 4096 f32       9.6 us: latency (launch and codes 2, set-up 1.3, first weights 1.2, weights 2.6,
+//   1 x 4096 x 4096 f32       9.5 us: latency (launch and codes 2, set-up 1.3, first weights 1.2, weights 2.6,
 //                             joining 1)
 // What the steps gave: loads announced without release semantics 291 -> 191 us at the largest size; MMAs
 // issued by a converged warp 383 -> 183 clocks per unit; no local memory in the epilogue 264 -> 215 k clocks;

@@ -517,7 +517,11 @@ int submit(SmithEncoder* enc, cudaEvent_t e0, cudaEvent_t e1) {
       if (prm[4] < 1 || prm[0] % prm[4]) return fail("%s: %u rows are no multiple of fan = %u", name, prm[0], prm[4]);
       g.fan = (int)prm[4], a_rows = prm[0] / prm[4];
     }
-    if (g.rows == 0) return 0;
+    if (g.rows == 0) {               // nothing to launch; a timed submit still finds its events
+      if (e0) CU_TRY(cudaEventRecord(e0, c->stream));
+      if (e1) CU_TRY(cudaEventRecord(e1, c->stream));
+      return 0;
+    }
     const void* v = nullptr;
     void* out = nullptr;
     bool back = false;

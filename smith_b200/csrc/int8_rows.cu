@@ -206,11 +206,11 @@ __device__ __forceinline__ void make_codes(const uint4& raw, const Coder& coder,
 // longer row has beyond is read again.
 //
 // Many rows are bound by reading them and by instructions (about six per value), few by latency: two vectors
-// per thread serve both.  (4096 rows of 4096 f16: 15 us, 3.4 TB/s of reads and writes; four vectors and half
-// the threads 16, both between launches of the product.  One row of 4096 f32, until the product could begin: 128 threads 5.6 us, 256 threads 3.1,
-// 512 threads 1.5.)  At most 32 registers a thread, so that a block of the product finds room beside: a
-// quarter of an SM's register file holds three of its eleven warps, and with more registers here the SMs
-// that hold one of these blocks began the product 2.5 to 5 us late.
+// per thread serve both.  (4096 rows of 4096 f16: 15 to 16 us, 3.3 TB/s of reads and writes; four vectors and
+// half the threads 16 to 17.  One row of 4096 f32, until the product could begin: 128 threads 5.6 us, 256
+// threads 3.1, 512 threads 1.5.)  At most 32 registers a thread, so that a block of the product finds room
+// beside: a quarter of an SM's register file holds three of its eleven warps, and with more registers here
+// the SMs that hold one of these blocks began the product 2.5 to 5 us late.
 constexpr int kNearPlaces = 32, kHeld = 2, kMostThreads = 1024;
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kMostThreads, 2)

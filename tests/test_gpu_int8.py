@@ -482,6 +482,21 @@ def test_profiled_operators_report_their_kernels():
     assert entry["calls"] == 1 and entry["tflops"] >= 0 and entry["gbs"] > 0
 
 
+def test_profiling_takes_empty_batches():
+    """No rows: nothing is launched, and the timed submit reports it like any other."""
+    rec = smith.quantizeInt8(smith.tensorFrom(np.ones((64, 32), np.float32), [64, 32]))
+    ids = smith.create([0], "i32")
+
+    def calls():
+        groups = smith.groupRows(ids, 1)
+        return smith.matmulInt8(smith.create([0, 64]), rec), smith.matmulInt8Grouped(smith.create([0, 64]), rec, groups), groups
+
+    res = smith.profileFn(calls)
+    one, two, groups = res["result"]
+    assert one.shape == [0, 32] and two.shape == [0, 32] and smith.toNumpy(groups.offsets).tolist() == [0, 0]
+    assert {k["kernel"] for k in res["kernels"]} == {"matmul_int8", "matmul_int8_grouped", "group_rows"}
+
+
 def test_packed_weights_on_disk(tmp_path):
     a, w = data(3, 6, 130, 200, np.float32, experts=None)
     rec = smith.quantizeInt8(smith.tensorFrom(w, [130, 200]))
